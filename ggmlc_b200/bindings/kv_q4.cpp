@@ -3,12 +3,13 @@
 // stream and calls the C ABI; a decode step's calls are a few microseconds long, so none of that is
 // left to the interpreter (the same in Python took 8 to 12 us a call, here 3 to 5).
 #include <ATen/cuda/EmptyTensor.h>
-#include <ATen/ops/zeros.h>
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <optional>
@@ -118,10 +119,7 @@ class Cache {
         }
         const cudaStream_t st = stream();
         const size_t need = gb_kv_q4_attend_workspace_bytes(&c_, n, q.size(1));
-        at::Tensor& work = work_[st];  // split scratch, one per stream
-        if (!work.defined() || (size_t)work.numel() < need)
-            // the counters at its start are zero before first use and after every call
-            work = at::zeros({(int64_t)need}, k_.options());
+        const at::Tensor& work = scratch(st, (int64_t)need);
         check(gb_kv_q4_attend(&c_, &r, type_id(q.scalar_type()), q.data_ptr(), q.stride(0),
                               q.stride(1), q.size(1), max_kv,
                               (float)scale.value_or(1.0 / std::sqrt((double)c_.head_dim)),
@@ -140,6 +138,28 @@ class Cache {
   private:
     cudaStream_t stream() const {
         return c10::cuda::getCurrentCUDAStream(k_.device().index()).stream();
+    }
+
+    // Split scratch, one per stream: its calls run one after the other.  A call under capture never
+    // gets the memory of eager calls, which a larger call replaces, nor another capture's, which may
+    // replay at the same time or before it: each capture has its own, from the graph's pool, whose
+    // counters its first call zeroes as a node of that graph.  The pool keeps it for as long as the
+    // graph lives, also after the next capture on the stream has taken its place here.
+    const at::Tensor& scratch(cudaStream_t st, int64_t need) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        unsigned long long id = 0;
+        if (cudaStreamGetCaptureInfo(st, &status, &id) != cudaSuccess)
+            throw std::runtime_error("Q4KVCache: the stream's capture status cannot be read");
+        Scratch& s = work_[st];
+        const bool capturing = status == cudaStreamCaptureStatusActive;
+        at::Tensor& work = capturing ? s.captured : s.eager;
+        if (!work.defined() || work.numel() < need || (capturing && s.capture != id)) {
+            work = at::empty({need}, k_.options());
+            // the counters are zero before the first call and after every one
+            work.narrow(0, 0, std::min<int64_t>(need, GB_KV_Q4_WORK_ZEROED)).zero_();
+            if (capturing) s.capture = id;
+        }
+        return work;
     }
 
     int64_t rows_of(const at::Tensor& x, int64_t heads, const char* what) const {
@@ -192,7 +212,11 @@ class Cache {
     at::Tensor k_, v_;
     std::optional<at::Tensor> pages_;
     gb_kv_q4 c_{};
-    std::map<cudaStream_t, at::Tensor> work_;
+    struct Scratch {
+        at::Tensor eager, captured;
+        unsigned long long capture = 0;  // the capture `captured` belongs to
+    };
+    std::map<cudaStream_t, Scratch> work_;
 };
 
 }  // namespace

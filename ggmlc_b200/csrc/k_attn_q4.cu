@@ -49,6 +49,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "../../include/ggmlc_b200.h"
 #include "common.h"
 #include "kernels.h"
 #include "kq4.cuh"
@@ -197,6 +198,7 @@ struct Segment {
 // CTAs of one launch: the machine filled once.  The workspace: 3 counters per CTA, then 4 partials
 constexpr int kMaxCtas = 1024, kMaxCtasPerSm = 4;
 constexpr int64_t kCounterBytes = 3 * kMaxCtas * 4;
+static_assert(kCounterBytes <= GB_KV_Q4_WORK_ZEROED, "the counters are what callers zero");
 constexpr int64_t partial_floats(int64_t hd) { return kHeads * (hd + 2); }
 
 // whether this CTA is the last of n to arrive at the counter (which it then resets); what the

@@ -426,7 +426,8 @@ struct RopeKvQ4Args {
 void launch_rope_kv_q4(const RopeKvQ4Args& a, cudaStream_t st);
 // Attention of q rows over the cache: row r sees positions 0 .. min(pos, max_kv - 1) of its slot;
 // a row that sees none gets zeros.  o: contiguous [n][Hq][hd] of q's type.  work:
-// attn_q4_workspace bytes, zeroed before its first use (every launch leaves its counters zero).
+// attn_q4_workspace bytes, GB_KV_Q4_WORK_ZEROED of them zeroed before its first use (every launch
+// leaves its counters zero).
 struct AttnQ4Args {
     KvQ4 c;
     KvQ4Rows r;

@@ -3,7 +3,8 @@
 ``Q4KVCache`` wraps the two device buffers of a cache (and its page table) as torch tensors and
 runs the operators of ``libggmlc_b200.so`` on them (``gb_kv_q4_*``, include/ggmlc_b200.h, which
 documents the format).  Every call runs on the current CUDA stream of the cache's device and
-returns without waiting.
+returns without waiting.  Calls may be captured by ``torch.cuda.graph``; a graph's scratch is its own,
+so graphs may be replayed in any order and side by side.
 
     cache = Q4KVCache.empty(n_pages=64, n_kv_heads=8, page_len=256, head_dim=128,
                             pages=torch.tensor([[3, 7], [1, 5]], dtype=torch.int32, device="cuda"))

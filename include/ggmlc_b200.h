@@ -428,7 +428,10 @@ int gb_kv_q4_read(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, void*
  * anything (NaN included).  o: contiguous [n][Hq][head_dim] of q's type.  head_dim 64, 128 or 256.
  * Arithmetic: f32 q to about 1e-6 of fp32 (two-term f16 products, fp32 sums); f16 / bf16 q: V and
  * the probabilities rounded to f16, fp32 sums.  work: gb_kv_q4_attend_workspace_bytes() of device
- * memory (256-byte aligned), zeroed before its first use and then kept; calls that can overlap need one each. */
+ * memory (256-byte aligned), its first GB_KV_Q4_WORK_ZEROED bytes zeroed before the first use (every
+ * call leaves them zero); calls that can overlap, replays of captured graphs among them, need one
+ * each, and memory that a graph has captured has to outlive it. */
+#define GB_KV_Q4_WORK_ZEROED 16384
 size_t gb_kv_q4_attend_workspace_bytes(const gb_kv_q4* cache, int64_t n_rows, int64_t Hq);
 int gb_kv_q4_attend(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, const void* q,
                     int64_t q_row_stride, int64_t q_head_stride, int64_t Hq, int64_t max_kv,
