@@ -24,6 +24,8 @@
 //   V: (n - 8) * d in f16, one rounding (16-bit types); f32: that and the exact remainder as a
 //      second f16 term.  Scales of positions past n_r are replaced by zero, and their scores by
 //      -inf, by selection: what the memory holds there (NaN included) is never multiplied in.
+//      Packed positions see different numbers of keys: a key that only some of them see and whose
+//      V scale is no number gets scale zero, and the columns that see it get their NaN by addition.
 //   P: exp2(s - m + 14) in f16 (two terms for f32 and f16 outputs); the factor 2^14 cancels in O / l and
 //      keeps small probabilities out of f16's subnormals.
 //
@@ -47,6 +49,7 @@
 // us, of which an empty launch is 2.2.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "../../include/ggmlc_b200.h"
@@ -647,7 +650,7 @@ __global__ void __launch_bounds__(Shape<HD, PREC>::kWarps * 32, Shape<HD, PREC>:
         for (int step = sg.begin + warp; step < sg.end; step += kWarps) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
             __syncwarp();  // every lane's copies of this stage have landed
-            const uint8_t* st = smem + (warp * S::kStages + stage) * S::kStage;
+            uint8_t* st = smem + (warp * S::kStages + stage) * S::kStage;
             const uint32_t ok = oks >> (stage * NG) & ((1u << NG) - 1);
             const int valid = n - step * KEYS;  // < 1 for a row that sees nothing
             const bool all = n_first - step * KEYS >= KEYS && ok == (1u << NG) - 1;
@@ -742,6 +745,24 @@ __global__ void __launch_bounds__(Shape<HD, PREC>::kWarps * 32, Shape<HD, PREC>:
                     o[i][0] *= k0, o[i][1] *= k1, o[i][2] *= k0, o[i][3] *= k1;
                 m0 = x0, m1 = x1;
             }
+            int bad_key = INT_MAX;  // PACK: the first such key of the lane's block
+            bool any_bad = false;
+            if (PACK && step * KEYS + KEYS > n_first) {
+                // at most 7 keys; lanes c of a quad look at two each
+                const int k0 = max(n_first - step * KEYS, 0) + c, end = min(valid, KEYS);
+                uint16_t* sc = (uint16_t*)(st + 2 * S::kCode + S::kScale) + g * (HD / 8) / 32;
+                const bool b0 = k0 < end && bad_scales(sc[k0 * NB]);
+                const bool b1 = k0 + 4 < end && bad_scales(sc[(k0 + 4) * NB]);
+                any_bad = __any_sync(0xffffffffu, b0 || b1);  // every lane has read
+                if (any_bad) {
+                    if (b0) sc[k0 * NB] = 0;
+                    if (b1) sc[(k0 + 4) * NB] = 0;
+                    bad_key = b0 ? step * KEYS + k0 : b1 ? step * KEYS + k0 + 4 : INT_MAX;
+                    bad_key = min(bad_key, __shfl_xor_sync(0xffffffffu, bad_key, 1));
+                    bad_key = min(bad_key, __shfl_xor_sync(0xffffffffu, bad_key, 2));
+                    __syncwarp();
+                }
+            }
 #pragma unroll
             for (int q = 0; q < NG; ++q) {
                 float p[4];
@@ -807,6 +828,14 @@ __global__ void __launch_bounds__(Shape<HD, PREC>::kWarps * 32, Shape<HD, PREC>:
                             }
                         }
                     }
+                }
+            }
+            if (PACK && any_bad) {
+                const float nan = __int_as_float(0x7FFFFFFF);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if (bad_key < n0) o[i][0] = nan, o[i][2] = nan;
+                    if (bad_key < n1) o[i][1] = nan, o[i][3] = nan;
                 }
             }
             if (++stage == S::kStages) stage = 0;

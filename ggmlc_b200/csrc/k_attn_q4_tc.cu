@@ -11,6 +11,9 @@
 //   K, V: (code - 8) * scale in f16, one rounding; for f16 calls K as the sum of two f16 terms, which
 //   is exact (Q once more).  Measured at 333 tokens at 1999: 68 -> 83 us, and the error against 64
 //   bits from 3.3e-4 to 2.6e-4 where rounding the output alone makes 2.1e-4.
+//   V of a key that only some rows of the CTA see must not reach the others through 0 x NaN: there a
+//   scale that is no number is decoded as zero, and the first such key of each block of 32 dims kept;
+//   rows that see it get NaN in the block when they are written.
 //   q: f16 after a power of two per row, the largest element in [1, 2) (exact for bf16 but for
 //   elements 2^-14 below it); the factor returns in the softmax scale.
 //   P: exp2(s - m + 7) in f16, for f16 outputs as the sum of two f16 terms (V once more).  m is a
@@ -38,6 +41,7 @@
 // Every wait is bounded: one that runs out sets the error word and the CTA leaves without output.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "common.h"
@@ -273,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         p_full[2][2], q_full[2], o_most[2], o_full[2], all_done;
     __shared__ __align__(16) uint32_t s_ok[kOkRing][4];
     __shared__ uint32_t s_tmem;
+    __shared__ int s_bad[NB];  // per block of V: the first key whose scale was no number
     __shared__ float s_qs[2 * kRows];  // softmax scale of the rows in powers of two
     __shared__ int s_abort;
     volatile int* abort = &s_abort;
@@ -303,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int steps = max(tiles[0], tiles[1]);
 
+    if (tid < NB) s_bad[tid] = INT_MAX;
     if (tid == 0) {
         s_abort = 0;
         for (int i = 0; i < 2; ++i) {
@@ -443,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
             // thread: 8 keys 8 kg.. (of one group of 16: one page), words VW vw..
             const int kg = p & 15, vw = p >> 4;
+            const int all_see = limit(row0);  // keys below it are seen by every row
             struct Words {
                 uint32_t w[8][VW], s[8];
                 int keys;  // of the 8 keys, how many are seen
@@ -468,10 +475,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                         x.s[i] = __ldg(ds + i * NB);
                     }
                 },
-                [&](int j, const Words& x) {
+                [&](int j, Words& x) {
                     const int st = j & 1;
                     if (j >= 2 && !mbar_wait(&v_empty[st], ((j >> 1) - 1) & 1, abort)) return false;
                     uint8_t* dst = sV + st * S::kTileK + (kg >> 3) * (HD * 128);
+                    const int k0 = (first + j) * kKeys + kg * 8;
+                    if (k0 + 8 > all_see) {
+#pragma unroll
+                        for (int i = 7; i >= 0; --i) {
+                            if (!bad_scales(x.s[i])) continue;
+                            x.s[i] = 0;
+                            if (i < x.keys) atomicMin(&s_bad[vw * VW / 4], k0 + i);
+                        }
+                    }
                     __half2 vd[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -823,6 +839,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0;
+                }
+                if (lim > s_bad[c]) {  // (V's warps are done: their last stage has been multiplied)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0x7FFFFFFFu;
                 }
                 if (row < row1 && alone) {
                     constexpr int N = 16 / sizeof(T);

@@ -24,6 +24,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Scales that V's product cannot take: infinities, NaN and magnitudes beyond 8188, the largest that a
+// write stores (8 times more has no f16).  Their sign bits mark them, in each half of a word.
+__device__ __forceinline__ uint32_t bad_scales(uint32_t d) {
+    return ((d & 0x7FFF7FFFu) + 0x10001000u) & 0x80008000u;
+}
+
 // (x & MASK) | 0x64006400 as the one instruction it is (written in C it came out as two)
 template <uint32_t MASK>
 __device__ __forceinline__ uint32_t and_or(uint32_t x) {

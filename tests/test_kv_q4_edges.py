@@ -99,3 +99,51 @@ def test_graphs_replayed_side_by_side():
         torch.cuda.synchronize()
         for out, w in zip(outs, want):
             check(torch, out, *w)
+
+
+# ---- values that must not be seen --------------------------------------------------------------------
+# (KV heads, q heads of each, head_dim, rows, positions before them): rows of 128 or 256 on the tensor
+# cores' tiles for the 16-bit types, single rows, rows packed by 2, 4 and 8 positions
+CHUNKS = [(4, 8, 128, 300, 260), (8, 4, 128, 100, 0), (2, 3, 64, 400, 77), (1, 16, 64, 150, 2000),
+          (2, 8, 128, 20, 100), (2, 2, 64, 9, 20), (2, 1, 128, 21, 0), (1, 4, 256, 13, 60)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv, rk, hd, s, past", CHUNKS)
+def test_chunk_with_values_that_are_no_numbers(dtype, hkv, rk, hd, s, past):
+    """NaN in a block of V at some positions of the chunk: rows that see one have NaN in its 32 dims,
+    earlier rows and other dims are as ever."""
+    torch = _torch()
+    cache = make_cache(torch, 1, -(-(past + s) // 48), hkv, 48, hd, True, 43)
+    fill(torch, cache, [past + s], 44)
+    gen = torch.Generator().manual_seed(45)
+    for at, dim, head in ((past + s - 2, 3, 0), (past + s // 2, 40, hkv - 1), (past + 1, hd - 1, 0)):
+        x = torch.randn(1, hkv, hd, generator=gen).cuda()
+        y = x.clone()
+        y[0, head, dim] = math.nan
+        cache.write(x, y, at, 0)
+    held = [tuple(x.double() for x in cache.read(0, 0, rows=past + s))]
+    q = torch.randn(s, hkv * rk, hd, generator=gen).to(getattr(torch, dtype)).cuda()
+    want, tol = expect(torch, q, held, range(past, past + s), [0] * s, 1 / math.sqrt(hd))
+    assert not want[0].isnan().any() and want[-1].isnan().any()
+    got = cache.attend(q, past, 0)
+    check(torch, got, want, tol)
+    assert torch.equal(got.nan_to_num(9.0), cache.attend(q, past, 0).nan_to_num(9.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv, rk, hd, s, past", CHUNKS)
+def test_chunk_whose_later_positions_are_unwritten(dtype, hkv, rk, hd, s, past):
+    """The memory behind the later positions of a chunk holds whatever it held (scales that are
+    infinite, NaN, or too large for f16 times a code): rows before them do not notice."""
+    torch = _torch()
+    cache = make_cache(torch, 1, -(-(past + s) // 48), hkv, 48, hd, True, 47)
+    n = past + s // 2
+    held = fill(torch, cache, [n], 48)
+    q = torch.randn(s, hkv * rk, hd, generator=torch.Generator().manual_seed(49))
+    q = q.to(getattr(torch, dtype)).cuda()
+    rows = n - past
+    want, tol = expect(torch, q[:rows], held, range(past, n), [0] * rows, 1 / math.sqrt(hd))
+    check(torch, cache.attend(q, past, 0)[:rows], want, tol)
