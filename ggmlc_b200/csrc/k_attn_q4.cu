@@ -588,13 +588,14 @@ __global__ void __launch_bounds__(Shape<HD, PREC>::kWarps * 32, Shape<HD, PREC>:
             bad += __shfl_xor_sync(0xffffffffu, bad, 2);
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // 2^e with big / 2^e in [1, 2).  A head with an infinity or a NaN has NaN scores
+            // 2^e with big / 2^e in [1, 2).  A head with an infinity or a NaN is NaN throughout: it has
+            // NaN scores where it sees a key, and its masked scores stay -inf
             const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -126), 126);
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
             float down = __uint_as_float((uint32_t)(127 - e) << 23);
             // a negative scale moves into q, a zero one becomes too small to tell scores apart: qs is
             // positive, so the largest raw sum is the largest score
-            qs = fmaxf(fabsf(a.scale) * kLog2e * up, 1e-30f) + bad;
+            qs = fmaxf(fabsf(a.scale) * kLog2e * up, 1e-30f);
             if (a.scale < 0.0f) down = -down;
             auto pack = [&](float u, float v) { return h2u(__floats2half2_rn(u, v)); };
             float term[2];  // off of blocks b - 1, b: the c-th f16 term
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(Shape<HD, PREC>::kWarps * 32, Shape<HD, PREC>:
             for (int b = 0; b < NB; ++b) {
                 float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[b][j] *= down;
+                for (int j = 0; j < 8; ++j) x[b][j] = fmaf(x[b][j], down, bad);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float u = x[b][j], v = x[b][j + 4];

@@ -666,17 +666,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                         bad += __shfl_xor_sync(0xffffffffu, bad, o);
                     }
                     // 2^e with big / 2^e in [1, 2); a negative scale moves into q, a zero one
-                    // becomes too small to tell scores apart
+                    // becomes too small to tell scores apart.  A row with an infinity or a NaN is
+                    // NaN throughout: NaN scores where it sees a key, and -inf where it does not
                     const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -126), 126);
                     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                     float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    if (w == 0) s_qs[r] = fmaxf(fabsf(a.scale) * kLog2e * up, 1e-30f) + bad;
+                    if (w == 0) s_qs[r] = fmaxf(fabsf(a.scale) * kLog2e * up, 1e-30f);
                     if (a.scale < 0.0f) down = -down;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = fmaf(y[j], down, bad);
                     uint4 v;
-                    v.x = h2u(__floats2half2_rn(y[0] * down, y[4] * down));
-                    v.y = h2u(__floats2half2_rn(y[1] * down, y[5] * down));
-                    v.z = h2u(__floats2half2_rn(y[2] * down, y[6] * down));
-                    v.w = h2u(__floats2half2_rn(y[3] * down, y[7] * down));
+                    v.x = h2u(__floats2half2_rn(y[0], y[4]));
+                    v.y = h2u(__floats2half2_rn(y[1], y[5]));
+                    v.z = h2u(__floats2half2_rn(y[2], y[6]));
+                    v.w = h2u(__floats2half2_rn(y[3], y[7]));
                     const int rt = r & (kRows - 1);
                     *(uint4*)(sQ + (r >> 7) * S::kTileK + rt * 128 + (w >> 3) * (kRows * 128) +
                               (((w & 7) ^ (rt & 7)) << 4)) = v;

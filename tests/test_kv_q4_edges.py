@@ -147,3 +147,31 @@ def test_chunk_whose_later_positions_are_unwritten(dtype, hkv, rk, hd, s, past):
     rows = n - past
     want, tol = expect(torch, q[:rows], held, range(past, n), [0] * rows, 1 / math.sqrt(hd))
     check(torch, cache.attend(q, past, 0)[:rows], want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_rows_that_see_nothing_are_zero_whatever_q_holds(dtype, bad):
+    """Padding rows (position -1, a slot or pages outside the cache), also those that share a tile or a
+    group with rows that see keys: their q is not looked at.  Rows that see a key have no value."""
+    torch = _torch()
+    dt = getattr(torch, dtype)
+    cache = make_cache(torch, 3, 8, 4, 64, 128, True, 51)
+    held = fill(torch, cache, [400, 400, 0], 52)
+    cache.pages[2] = 1000
+    gen = torch.Generator().manual_seed(53)
+    for rows, heads in ((4, 32), (6, 8), (300, 32)):  # single, packed, tiles (16-bit types)
+        q = torch.randn(rows, heads, 128, generator=gen).to(dt).cuda()
+        q[:3, 1] = bad
+        q[1, :, 7] = bad
+        q[rows - 1, 5, 100] = bad
+        got = cache.attend(q, -3, 1)
+        assert not got[:3].any()
+        want, tol = expect(torch, q, held, range(-3, rows - 3), [1] * rows, 1 / math.sqrt(128))
+        assert want[rows - 1, 5].isnan().all()
+        check(torch, got, want, tol)
+        assert not cache.attend(q, 20, 2).any()
+        assert not cache.attend(q, 20, 7).any()
+        pos = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+        assert not cache.attend(q, pos, torch.zeros_like(pos)).any()
