@@ -94,6 +94,37 @@ bool kv_q4_type_ok(int type) {
     return type == gb::kTypeF32 || type == gb::kTypeF16 || type == gb::kTypeBF16;
 }
 
+// the checked arguments of an attention call over a 4-bit cache; max_kv: of the rows' sequences
+gb::AttnQ4Args attn_q4_of(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, const void* q,
+                          int64_t q_row, int64_t q_head, int64_t Hq, int64_t max_kv, float scale,
+                          void* o, void* work, size_t work_bytes, const std::string& what) {
+    gb::AttnQ4Args a;
+    a.c = kv_q4_of(cache, what);
+    a.r = kv_q4_rows_of(rows, what);
+    GB_CHECK(kv_q4_type_ok(type), what + ": type must be f32, f16 or bf16");
+    GB_CHECK(gb::attn_q4_head_dim(a.c.hd), what + ": head_dim must be 64, 128 or 256");
+    GB_CHECK(Hq > 0 && Hq <= 65536 && Hq % a.c.Hkv == 0,
+             what + ": Hq must be a multiple of n_kv_heads");
+    GB_CHECK(q_row >= 0 && q_head >= 0, what + ": strides must not be negative");
+    if (a.r.n == 0) return a;
+    GB_CHECK(q && o, what + ": q and o must not be NULL");
+    GB_CHECK(work && ((uintptr_t)work & 255) == 0 &&
+                 work_bytes >= gb::attn_q4_workspace(a.c.hd, a.r.n > 1),
+             what + ": work must be gb_kv_q4_attend_workspace_bytes() of 256-byte aligned device "
+                    "memory");
+    a.type = type;
+    a.q = q;
+    a.q_row = q_row;
+    a.q_head = q_head;
+    a.Hq = (int)Hq;
+    const int64_t cap = a.c.per_slot * a.c.page_len;
+    a.max_kv = max_kv > 0 && max_kv < cap ? max_kv : cap;
+    a.scale = scale;
+    a.o = o;
+    a.work = work;
+    return a;
+}
+
 gb_graph* wrap(std::shared_ptr<gb::Graph> g) {
     auto* h = new gb_graph();
     h->g = std::move(g);
@@ -831,34 +862,26 @@ int gb_kv_q4_attend(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, con
                     int64_t q_row_stride, int64_t q_head_stride, int64_t Hq, int64_t max_kv,
                     float scale, void* o, void* work, size_t work_bytes, void* stream) {
     return guard([&] {
-        gb::AttnQ4Args a;
-        a.c = kv_q4_of(cache, "gb_kv_q4_attend");
-        a.r = kv_q4_rows_of(rows, "gb_kv_q4_attend");
-        GB_CHECK(kv_q4_type_ok(type), "gb_kv_q4_attend: type must be f32, f16 or bf16");
-        GB_CHECK(gb::attn_q4_head_dim(a.c.hd), "gb_kv_q4_attend: head_dim must be 64, 128 or 256");
-        GB_CHECK(Hq > 0 && Hq <= 65536 && Hq % a.c.Hkv == 0,
-                 "gb_kv_q4_attend: Hq must be a multiple of n_kv_heads");
-        GB_CHECK(q_row_stride >= 0 && q_head_stride >= 0,
-                 "gb_kv_q4_attend: strides must not be negative");
-        if (a.r.n == 0) return;
-        GB_CHECK(q && o, "gb_kv_q4_attend: q and o must not be NULL");
-        GB_CHECK(work && ((uintptr_t)work & 255) == 0 &&
-                     work_bytes >= gb::attn_q4_workspace(a.c.hd, a.r.n > 1),
-                 "gb_kv_q4_attend: work must be gb_kv_q4_attend_workspace_bytes() of 256-byte "
-                 "aligned device memory");
-        a.type = type;
-        a.q = q;
-        a.q_row = q_row_stride;
-        a.q_head = q_head_stride;
-        a.Hq = (int)Hq;
-        const int64_t cap = a.c.per_slot * a.c.page_len;
-        a.max_kv = max_kv > 0 && max_kv < cap ? max_kv : cap;
+        gb::AttnQ4Args a = attn_q4_of(cache, rows, type, q, q_row_stride, q_head_stride, Hq, max_kv,
+                                      scale, o, work, work_bytes, "gb_kv_q4_attend");
         // a chunk's last row tells the host how far any row sees
         if (!a.r.pos) a.max_kv = std::max<int64_t>(1, std::min(a.max_kv, a.r.pos0 + a.r.n));
-        a.scale = scale;
-        a.o = o;
-        a.work = work;
-        gb::launch_attn_q4(a, (cudaStream_t)stream);
+        if (a.r.n > 0) gb::launch_attn_q4(a, (cudaStream_t)stream);
+    });
+}
+int gb_kv_q4_attend_prefill(const gb_kv_q4* cache, int64_t n_rows, const int64_t* step_pos,
+                            int64_t slot, const float* q, int64_t q_row_stride,
+                            int64_t q_head_stride, int64_t Hq, int64_t max_kv, float scale, float* o,
+                            void* work, size_t work_bytes, void* stream) {
+    return guard([&] {
+        const std::string what = "gb_kv_q4_attend_prefill";
+        const gb_kv_rows rows{n_rows, nullptr, 0, nullptr, slot};
+        gb::AttnQ4Args a = attn_q4_of(cache, &rows, gb::kTypeF32, q, q_row_stride, q_head_stride, Hq,
+                                      max_kv, scale, o, work, work_bytes, what);
+        GB_CHECK(step_pos, what + ": step_pos must not be NULL");
+        a.r.step_pos = step_pos;
+        a.fast_f32 = true;
+        if (a.r.n > 0) gb::launch_attn_q4(a, (cudaStream_t)stream);
     });
 }
 

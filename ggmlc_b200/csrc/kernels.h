@@ -442,8 +442,9 @@ struct AttnQ4Args {
     int shift = -1;      // set by the launchers: kv_q4_shift
     bool q_vec = false;  // set by the launchers: kv_q4_vectors
     int pack = 1;        // set by the launcher: positions of a chunk that share a row of work
-    // f32 q whose chunks may go through the f16 operands of the tcgen05 kernel (the engine's prefill,
-    // whose f16 cache rounds q and the probabilities alike); otherwise f32 keeps two-term products
+    // f32 q whose chunks may go through the f16 operands of the tcgen05 kernel: q, K and V rounded to
+    // f16, the probabilities in two terms (the engine's prefill; its attention over an f16 cache rounds
+    // q and the probabilities to f16 too); otherwise f32 keeps two-term products
     bool fast_f32 = false;
 };
 // q can be read in 16-byte pieces: its base and strides are whole ones
@@ -457,8 +458,8 @@ size_t attn_q4_tc_parts(int64_t hd);
 double attn_q4_tc_us(const AttnQ4Args& a);         // the chunk kernel's time, as its launch plans it
 bool attn_q4_head_dim(int64_t hd);  // head dims the attention kernels are built for
 void launch_attn_q4(const AttnQ4Args& a, cudaStream_t st);
-// The same for a chunk (pos and slot NULL) on tcgen05 (k_attn_q4_tc.cu): f16 / bf16 q, head_dim 64
-// or 128; launch_attn_q4 sends the chunks there that fill its tiles.  attn_q4_tc_error: its sticky
+// The same for a chunk (pos and slot NULL) on tcgen05 (k_attn_q4_tc.cu): f16 / bf16 q, f32 with
+// fast_f32, head_dim 64 or 128; launch_attn_q4 sends the chunks there that fill its tiles.  attn_q4_tc_error: its sticky
 // error word (non-zero after one of its bounded waits ran out).
 bool attn_q4_tc_fits(const AttnQ4Args& a);
 void launch_attn_q4_tc(const AttnQ4Args& a, cudaStream_t st);

@@ -49,7 +49,9 @@ for _name, _args, _res in (
         ("gb_kv_q4_write", [_P, _P, _I, _P, _I64, _I64, _P, _I64, _I64, _P], _I),
         ("gb_kv_q4_read", [_P, _P, _I, _P, _P, _P], _I),
         ("gb_kv_q4_attend_workspace_bytes", [_P, _I64, _I64], _SZ),
-        ("gb_kv_q4_attend", [_P, _P, _I, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ, _P], _I)):
+        ("gb_kv_q4_attend", [_P, _P, _I, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ, _P], _I),
+        ("gb_kv_q4_attend_prefill", [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ,
+                                     _P], _I)):
     getattr(_lib, _name).argtypes = _args
     getattr(_lib, _name).restype = _res
 

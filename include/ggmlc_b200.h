@@ -437,6 +437,15 @@ size_t gb_kv_q4_attend_workspace_bytes(const gb_kv_q4* cache, int64_t n_rows, in
 int gb_kv_q4_attend(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, const void* q,
                     int64_t q_row_stride, int64_t q_head_stride, int64_t Hq, int64_t max_kv,
                     float scale, void* o, void* work, size_t work_bytes, void* stream);
+/* The form of it that the engine's prefill runs over a 4-bit cache: f32 rows at positions *step_pos,
+ * *step_pos + 1, .. of sequence `slot`, step_pos a device int64 that a captured graph reads anew at
+ * each replay, and n_rows consecutive rows.  Arithmetic: chunks that the tensor cores' tiles take
+ * (head_dim 64 or 128) round q, K and V to f16 and keep the probabilities in two f16 terms, fp32
+ * sums; other calls are as above.  work as for gb_kv_q4_attend. */
+int gb_kv_q4_attend_prefill(const gb_kv_q4* cache, int64_t n_rows, const int64_t* step_pos,
+                            int64_t slot, const float* q, int64_t q_row_stride,
+                            int64_t q_head_stride, int64_t Hq, int64_t max_kv, float scale, float* o,
+                            void* work, size_t work_bytes, void* stream);
 /* Sticky error word of the chunk kernel: 0 while every bounded wait in it completed, non-zero after
  * one ran out (that call's output is not valid), -1 if the word cannot be read. */
 int gb_kv_q4_error(void);

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -175,3 +176,125 @@ def test_rows_that_see_nothing_are_zero_whatever_q_holds(dtype, bad):
         assert not cache.attend(q, 20, 7).any()
         pos = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
         assert not cache.attend(q, pos, torch.zeros_like(pos)).any()
+
+
+# ---- the engine's prefill form ----------------------------------------------------------------------
+class Prefill:
+    """gb_kv_q4_attend_prefill over a torch class's cache: f32 rows, the position read on the device."""
+
+    def __init__(self, torch, cache, hq, rows):
+        from ggmlc_b200 import kv_q4
+
+        self.lib, p = kv_q4._lib, cache.pages
+        self.cache = cache
+        self.c = kv_q4._Cache(cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0],
+                              cache.page_len, cache.n_kv_heads, cache.head_dim,
+                              p.data_ptr() if p is not None else None,
+                              p.shape[0] if p is not None else 0, p.shape[1] if p is not None else 0)
+        need = self.lib.gb_kv_q4_attend_workspace_bytes(ctypes.addressof(self.c), rows, hq)
+        self.work = torch.zeros(need, dtype=torch.uint8, device="cuda")
+        self.pos = torch.zeros(1, dtype=torch.int64, device="cuda")
+        self.hq, self.rows = hq, rows
+
+    def __call__(self, torch, q, out, slot=0, max_kv=0):
+        rc = self.lib.gb_kv_q4_attend_prefill(
+            ctypes.addressof(self.c), self.rows, self.pos.data_ptr(), slot, q.data_ptr(),
+            q.stride(0), q.stride(1), self.hq, max_kv, 1 / math.sqrt(self.cache.head_dim),
+            out.data_ptr(), self.work.data_ptr(), self.work.numel(),
+            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, self.lib.gb_last_error()
+
+
+def expect_prefill(torch, q, held, pos, slot):
+    """f64 attention and the bound of each element where q, K and V are rounded to f16 (2^-11 of each)
+    and the rest is f32: an error e in a score changes a probability by the factor exp(e), and e is at
+    most scale times the sum of |q| |k| (2^-11 + 2^-11), with 2^-24 of the row's largest |q| for the
+    elements that f16 does not hold beside it."""
+    hd, hkv = q.shape[2], held[slot][0].shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    for r in range(q.shape[0]):
+        k, v = (x[:pos + r + 1] for x in held[slot])
+        qr = q[r].double().reshape(hkv, -1, hd)
+        w = torch.softmax(torch.einsum("hgd,thd->hgt", qr, k) / math.sqrt(hd), -1)
+        out[r] = torch.einsum("hgt,thd->hgd", w, v).reshape(-1, hd)
+        off = qr.abs() * 2.0**-10 + qr.abs().amax(-1, keepdim=True) * 2.0**-24
+        e = torch.einsum("hgd,thd->hgt", off, k.abs()).amax(-1) / math.sqrt(hd)
+        absolute = torch.einsum("hgt,thd->hgd", w, v.abs()).reshape(-1, hd)
+        tol[r] = absolute * (2.0**-11 + 2.0**-18 + 2 * e).reshape(-1, 1) + 1e-12
+    return out, tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hkv, rk, hd", [(8, 4, 128), (8, 2, 64), (3, 3, 64), (2, 10, 128)])
+@pytest.mark.parametrize("s, past, capacity", [(512, 0, 512), (500, 0, 8192), (300, 333, 700),
+                                               (300, 333, 40000), (129, 2000, 4096), (512, 100, 640)])
+def test_prefill_form_on_tiles(hkv, rk, hd, s, past, capacity):
+    """Windows as wide as the chunk and far wider (the plan is made for the window, its runs of key
+    tiles are cut by the position, which only the device knows)."""
+    torch = _torch()
+    cache = make_cache(torch, 2, -(-capacity // 64), hkv, 64, hd, True, 61)
+    held = fill(torch, cache, [0, past + s], 62)
+    q = torch.randn(s, hkv * rk, hd, generator=torch.Generator().manual_seed(63)).cuda()
+    call, out = Prefill(torch, cache, hkv * rk, s), torch.empty_like(q)
+    call.pos.fill_(past)
+    call(torch, q, out, slot=1)
+    want, tol = expect_prefill(torch, q, held, past, 1)
+    check(torch, out, want, tol)
+    # independent errors: 2^-11 / sqrt(3) of V, and as much of q and K each times the spread of a score
+    # (1.1 here, keys of uneven channels up to 1.6), less than 1e-3 together; a tile left out or taken
+    # twice would show as some percent
+    err = float((out - want).norm() / want.norm())
+    assert err < 2e-3
+    # by rows, f32 stays below 1e-5: the tiles were what ran
+    assert err > 3e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("contiguous", [False, True])
+def test_prefill_form_in_a_graph_reads_the_position_anew(contiguous):
+    """One captured call over a window of 2048 replayed at several positions."""
+    torch = _torch()
+    hkv, rk, hd, s, cap = 8, 4, 64, 200, 2048
+    cache = make_cache(torch, 2, 1 if contiguous else cap // 64, hkv, cap if contiguous else 64, hd,
+                       not contiguous, 65)
+    held = fill(torch, cache, [0, cap], 66)
+    q = torch.randn(s, hkv * rk, hd, generator=torch.Generator().manual_seed(67)).cuda()
+    call, out = Prefill(torch, cache, hkv * rk, s), torch.empty_like(q)
+    call(torch, q, out, slot=1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(torch, q, out, slot=1)
+    for past in (0, 1, 120, 1000, cap - s, 0):
+        call.pos.fill_(past)
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(torch, out, *expect_prefill(torch, q, held, past, 1))
+    eager = torch.empty_like(q)
+    call(torch, q, eager, slot=1)
+    assert torch.equal(eager, out)
+
+
+def test_prefill_form_refusals():
+    from test_kv_q4 import _c_cache
+
+    from ggmlc_b200 import kv_q4 as kv
+
+    c, wide, p = _c_cache(kv), _c_cache(kv, head_dim=96), 1 << 23
+    L = kv._lib
+
+    def refused(word, cache=c, n=2, step=p, q=p, row=128, hq=2, o=p, work=p, size=1 << 30):
+        rc = L.gb_kv_q4_attend_prefill(ctypes.addressof(cache), n, step, 0, q, row, 64, hq, 0, 1.0, o,
+                                       work, size, None)
+        assert rc == -1 and word in L.gb_last_error().decode(), L.gb_last_error()
+
+    refused("rows", n=-1)
+    refused("multiple", hq=3)
+    refused("strides", row=-1)
+    refused("NULL", q=None)
+    refused("NULL", o=None)
+    refused("head_dim", cache=wide)
+    refused("work", work=None)
+    refused("work", work=p + 16)
