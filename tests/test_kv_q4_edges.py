@@ -4,9 +4,23 @@ from __future__ import annotations
 
 import ctypes
 import math
+import re
+from pathlib import Path
 
 import pytest
-from test_kv_q4 import DTYPES, _torch, check, expect, fill, make_cache
+from test_kv_q4 import DTYPES, _c_cache, _torch, check, expect, fill, make_cache
+
+from ggmlc_b200 import kv_q4
+
+
+# ---- what a kernel may read that starts before the one that writes it has ended -----------------------
+@pytest.mark.parametrize("source", ["k_attn_q4.cu", "k_attn_q4_tc.cu", "k_kv_q4.cu"])
+def test_no_read_only_loads(source):
+    """The cache's kernels start while the kernel before them may still run (programmatic dependent
+    launch); the read-only path is for memory that nobody writes while the kernel lives."""
+    code = (Path(kv_q4.__file__).parent / "csrc" / source).read_text()
+    code = re.sub(r"//[^\n]*", "", code)
+    assert "launch_pdl(" in code and not re.search(r"__ldg\b|ld\.global\.nc|__restrict__", code)
 
 
 # ---- captured graphs -------------------------------------------------------------------------------
@@ -183,8 +197,6 @@ class Prefill:
     """gb_kv_q4_attend_prefill over a torch class's cache: f32 rows, the position read on the device."""
 
     def __init__(self, torch, cache, hq, rows):
-        from ggmlc_b200 import kv_q4
-
         self.lib, p = kv_q4._lib, cache.pages
         self.cache = cache
         self.c = kv_q4._Cache(cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0],
@@ -278,12 +290,8 @@ def test_prefill_form_in_a_graph_reads_the_position_anew(contiguous):
 
 
 def test_prefill_form_refusals():
-    from test_kv_q4 import _c_cache
-
-    from ggmlc_b200 import kv_q4 as kv
-
-    c, wide, p = _c_cache(kv), _c_cache(kv, head_dim=96), 1 << 23
-    L = kv._lib
+    c, wide, p = _c_cache(kv_q4), _c_cache(kv_q4, head_dim=96), 1 << 23
+    L = kv_q4._lib
 
     def refused(word, cache=c, n=2, step=p, q=p, row=128, hq=2, o=p, work=p, size=1 << 30):
         rc = L.gb_kv_q4_attend_prefill(ctypes.addressof(cache), n, step, 0, q, row, 64, hq, 0, 1.0, o,
