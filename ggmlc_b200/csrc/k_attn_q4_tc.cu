@@ -510,24 +510,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (j >= 2 && !mbar_wait(&v_empty[st], ((j >> 1) - 1) & 1, abort)) return false;
                     uint8_t* dst = sV + st * S::kTileK + (kg >> 3) * (HD * 128);
                     const int k0 = (first + j) * kKeys + kg * 8;
-                    if (k0 + 8 > all_see) {
+                    if (x.keys < 8 || k0 + 8 > all_see) {
 #pragma unroll
                         for (int i = 7; i >= 0; --i) {
-                            if (!bad_scales(x.s[i])) continue;
+                            if (i < x.keys && !bad_scales(x.s[i])) continue;
                             x.s[i] = 0;
                             if (i < x.keys) atomicMin(&s_bad[vw * VW / 4], k0 + i);
                         }
                     }
                     __half2 vd[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t d = __byte_perm(x.s[2 * i], x.s[2 * i + 1], 0x5410);
-                        if (x.keys < 8) {
-                            if (2 * i >= x.keys) d = 0;
-                            if (2 * i + 1 >= x.keys) d &= 0xFFFF;
-                        }
-                        vd[i] = u2h(d);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        vd[i] = u2h(__byte_perm(x.s[2 * i], x.s[2 * i + 1], 0x5410));
 #pragma unroll
                     for (int i = 0; i < VW; ++i) {
 #pragma unroll
