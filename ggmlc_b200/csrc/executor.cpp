@@ -476,6 +476,22 @@ void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged) {
                      " bytes; raise tokens_per_page");
         pages += 1;  // + the scratch page 0
     }
+    // checked: from here on the present cache, if any, makes room for the new one; a layout that fails
+    // on the device leaves none
+    if (kv_enabled_) free_kv();
+    try {
+        alloc_kv_pools(caches, slots, max_ctx, paged, pages);
+    } catch (...) {
+        free_kv();
+        cudaGetLastError();  // the failed allocation is reported once
+        throw;
+    }
+    kv_max_ctx_ = max_ctx;
+    kv_enabled_ = true;
+}
+
+void Executor::alloc_kv_pools(std::map<uint32_t, KVCache>& caches, int64_t slots, int64_t max_ctx,
+                              int64_t paged, int64_t pages) {
     for (auto& [id, c] : caches) {
         c.elems = paged ? pages * c.Hkv * tokens_per_page_ * c.hd : c.hd * c.Hkv * slots * max_ctx;
         if (c.q4) {
@@ -483,11 +499,11 @@ void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged) {
             c.n_pages = paged ? pages : slots;
         }
         const size_t bytes = c.bytes();
-        GB_CUDA(cudaMalloc(&c.k, bytes));
-        GB_CUDA(cudaMalloc(&c.v, bytes));
-        GB_CUDA(cudaMemset(c.k, 0, bytes));
-        GB_CUDA(cudaMemset(c.v, 0, bytes));
-        kv_[id] = c;
+        KVCache& held = kv_[id] = c;  // what is allocated is free_kv's from here on
+        GB_CUDA(cudaMalloc(&held.k, bytes));
+        GB_CUDA(cudaMalloc(&held.v, bytes));
+        GB_CUDA(cudaMemset(held.k, 0, bytes));
+        GB_CUDA(cudaMemset(held.v, 0, bytes));
         if (c.q4 && !kv_q4_work_) {
             size_t work = 0;
             for (auto& [i2, c2] : caches) work = std::max(work, attn_q4_workspace(c2.hd, true));
@@ -517,8 +533,6 @@ void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged) {
         ptab_dirty_ = false;
         ++pool_gen_;
     }
-    kv_max_ctx_ = max_ctx;
-    kv_enabled_ = true;
 }
 
 void Executor::set_decode_chain(bool on) {
@@ -561,7 +575,6 @@ void Executor::free_kv() {
 void Executor::init_paged_kv_cache(int64_t max_batch, int64_t max_ctx) {
     GB_CHECK(max_batch >= 1 && max_batch <= kMaxRows, "paged KV: max_batch must be 1..16");
     GB_CHECK(max_ctx >= 1, "paged KV: max_ctx must be positive");
-    if (kv_enabled_) free_kv();
     alloc_kv(max_batch + 1, max_ctx, max_batch);  // + the scratch slot of padding rows
     GB_CHECK(kv_enabled_, "paged KV: the graph has no attention over a KV cache");
     paged_ = true;
@@ -732,9 +745,14 @@ void Executor::set_tokens_per_page(int64_t n) {
         return;
     }
     for (char live : slot_live_) GB_CHECK(!live, "tokens_per_page: a slot is in use");
-    const int64_t mb = paged_max_batch_, mc = paged_max_ctx_;
+    const int64_t mb = paged_max_batch_, mc = paged_max_ctx_, old = tokens_per_page_;
     tokens_per_page_ = n;
-    init_paged_kv_cache(mb, mc);  // the pool is laid out again (the prefix cache starts empty)
+    try {
+        init_paged_kv_cache(mb, mc);  // the pool is laid out again (the prefix cache starts empty)
+    } catch (...) {
+        tokens_per_page_ = old;
+        throw;
+    }
 }
 
 void Executor::prepare_batch(int rows, const int32_t* pos, const int32_t* slot) {

@@ -332,7 +332,10 @@ private:
     void ensure_arena(size_t bytes);
     // contiguous windows for `slots` sequences, or (paged > 0) page pools sized for `paged`
     // sequences plus the prefix pages (init_paged_kv_cache)
+    // lays out a cache in the place of the present one; a refused layout leaves that as it is
     void alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged = 0);
+    void alloc_kv_pools(std::map<uint32_t, KVCache>& caches, int64_t slots, int64_t max_ctx,
+                        int64_t paged, int64_t pages);
     void free_kv();
     bool logits_last_only_ = false;
     std::vector<int32_t> out_rows_;
