@@ -411,12 +411,14 @@ class ModelExecutor:
     def set_kv_cache_type(self, kv_type: str) -> None:
         """Type of the KV cache the next init_kv_cache / init_paged_kv_cache lays out (engine
         extension): "f16" (the default) or "q4_0", 4.5 bits a value, quantised as rows are
-        written (head_dim 64, 128 or 256; tokens_per_page of at least 16; one GPU)."""
+        written (head_dim 64, 128 or 256; tokens_per_page of at least 16; one GPU).
+        init_kv_cache replaces a contiguous cache of the other type by an empty one."""
         if kv_type not in _KV_TYPES:
             raise ValueError(f"KV cache type must be one of {sorted(_KV_TYPES)}, got {kv_type!r}")
         _check(_lib.gb_executor_set_kv_cache_type(self._h, _KV_TYPES[kv_type]))
 
     def kv_cache_type(self) -> str:
+        """Type of the KV cache that is held, or of the next one while there is none."""
         t = int(_lib.gb_executor_kv_cache_type(self._h))
         return next(k for k, v in _KV_TYPES.items() if v == t)
 

@@ -413,11 +413,14 @@ void Executor::upload_weights() {
 // ------------------------------------------------------------------------------ KV cache
 
 void Executor::init_kv_cache(int64_t max_ctx) {
-    if (kv_enabled_) return;
+    if (kv_enabled_ && kv_type_ == kv_type_want_) return;
+    GB_CHECK(!paged_, "a paged KV cache of another type is in place: init_paged_kv_cache lays out a "
+                      "new one");
     alloc_kv(1, max_ctx);
 }
 
-void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged) {
+void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged, int type) {
+    if (type < 0) type = kv_type_want_;
     // enable rule of the reference (executor.cpp:505-539)
     bool has_rope = false, has_pos_sym = false, has_pos_in = false, has_arange = false;
     for (auto& op : g_->ops) has_rope |= op.opcode == OP_ROPE;
@@ -445,7 +448,7 @@ void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged) {
         c.ctx = max_ctx;
         c.slots = slots;
         GB_CHECK(c.batch == 1, "KV caches with a graph batch dimension are not supported");
-        c.q4 = kv_type_want_ == T_Q4_0;
+        c.q4 = type == T_Q4_0;
         if (c.q4) {
             GB_CHECK(tp_.size == 1, "a 4-bit KV cache runs on one GPU");
             GB_CHECK(attn_q4_head_dim(c.hd), "a 4-bit KV cache needs head_dim 64, 128 or 256");
@@ -487,6 +490,7 @@ void Executor::alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged) {
         throw;
     }
     kv_max_ctx_ = max_ctx;
+    kv_type_ = type;
     kv_enabled_ = true;
 }
 
@@ -573,9 +577,13 @@ void Executor::free_kv() {
 }
 
 void Executor::init_paged_kv_cache(int64_t max_batch, int64_t max_ctx) {
+    init_paged(max_batch, max_ctx, kv_type_want_);
+}
+
+void Executor::init_paged(int64_t max_batch, int64_t max_ctx, int type) {
     GB_CHECK(max_batch >= 1 && max_batch <= kMaxRows, "paged KV: max_batch must be 1..16");
     GB_CHECK(max_ctx >= 1, "paged KV: max_ctx must be positive");
-    alloc_kv(max_batch + 1, max_ctx, max_batch);  // + the scratch slot of padding rows
+    alloc_kv(max_batch + 1, max_ctx, max_batch, type);  // + the scratch slot of padding rows
     GB_CHECK(kv_enabled_, "paged KV: the graph has no attention over a KV cache");
     paged_ = true;
     paged_max_batch_ = max_batch;
@@ -748,7 +756,8 @@ void Executor::set_tokens_per_page(int64_t n) {
     const int64_t mb = paged_max_batch_, mc = paged_max_ctx_, old = tokens_per_page_;
     tokens_per_page_ = n;
     try {
-        init_paged_kv_cache(mb, mc);  // the pool is laid out again (the prefix cache starts empty)
+        // the pool is laid out again, in the type it has (the prefix cache starts empty)
+        init_paged(mb, mc, kv_type_);
     } catch (...) {
         tokens_per_page_ = old;
         throw;

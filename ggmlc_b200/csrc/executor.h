@@ -202,9 +202,11 @@ public:
     int64_t kv_page_bytes() const;   // one page: T positions of K and V in every layer
     void configure_prefix_pool(int64_t pages);  // prefix-cache pages beyond max_batch sequences
     void configure_kv_pool_pages(int64_t pages);  // explicit pool size (0: the default rule)
-    // T_F16 (the default) or T_Q4_0: the cache held in 4 bits (KvQ4); takes effect at the next init
+    // T_F16 (the default) or T_Q4_0: the cache held in 4 bits (KvQ4); takes effect at the next init,
+    // which replaces a contiguous cache of the other type.  kv_cache_type: of the cache that is held,
+    // or, before there is one, of the next
     void set_kv_cache_type(int type);
-    int kv_cache_type() const { return kv_type_want_; }
+    int kv_cache_type() const { return kv_enabled_ ? kv_type_ : kv_type_want_; }
     int64_t kv_pool_pages() const;   // pages sequences and the prefix cache can use
     int64_t kv_free_pages() const;   // pages nobody references
     int64_t paged_kv_slot_pages(int64_t slot) const;  // pages in the slot's table
@@ -301,7 +303,7 @@ private:
     size_t weight_bytes_ = 0;
     std::map<uint32_t, KVCache> kv_;    // per FLASH_ATTN_EXT op id
     bool kv_enabled_ = false;
-    int kv_type_want_ = T_F16;
+    int kv_type_want_ = T_F16, kv_type_ = T_F16;  // of the next layout, of the one that is held
     void* kv_q4_work_ = nullptr;  // split scratch of 4-bit cache attention (its counters zeroed once)
     int64_t kv_max_ctx_ = 0;
     bool paged_ = false;
@@ -333,7 +335,8 @@ private:
     // contiguous windows for `slots` sequences, or (paged > 0) page pools sized for `paged`
     // sequences plus the prefix pages (init_paged_kv_cache)
     // lays out a cache in the place of the present one; a refused layout leaves that as it is
-    void alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged = 0);
+    void alloc_kv(int64_t slots, int64_t max_ctx, int64_t paged = 0, int type = -1);
+    void init_paged(int64_t max_batch, int64_t max_ctx, int type);
     void alloc_kv_pools(std::map<uint32_t, KVCache>& caches, int64_t slots, int64_t max_ctx,
                         int64_t paged, int64_t pages);
     void free_kv();

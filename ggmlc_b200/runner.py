@@ -159,7 +159,8 @@ class ModelRunner:
 
     def init_kv_cache(self, max_ctx: int = 2048, kv_type: str | None = None) -> None:
         """``kv_type`` "f16" or "q4_0" (engine extension): the cache's type, the executor's present
-        choice when None."""
+        choice when None.  A cache of that type is kept as it is, one of the other replaced by an
+        empty one."""
         if kv_type is not None:
             self.executor.set_kv_cache_type(kv_type)
         self.executor.init_kv_cache(max_ctx)

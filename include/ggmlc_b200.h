@@ -114,7 +114,9 @@ int gb_executor_has_kv_cache(const gb_executor* e);
 /* Type of the KV cache the next init_kv_cache / init_paged_kv_cache lays out (engine extension, no
  * reference twin): 1 f16 (the default) or 2 q4_0, the cache held in 4 bits described below (4.5
  * bits a value; head_dim 64, 128 or 256, tokens_per_page of at least 16, one GPU).  Prefills and
- * decode steps then quantise their K and V rows as they write them. */
+ * decode steps then quantise their K and V rows as they write them.  gb_executor_init_kv_cache
+ * replaces a contiguous cache of the other type by an empty one; over a paged one it is an error.
+ * gb_executor_kv_cache_type: the type of the cache that is held, of the next while there is none. */
 int gb_executor_set_kv_cache_type(gb_executor* e, int type);
 int gb_executor_kv_cache_type(const gb_executor* e);
 /* set_logits_last_only / logits_last_only — executor.cpp:2398-2410 */

@@ -86,3 +86,48 @@ def test_a_layout_that_does_not_fit_leaves_nothing_behind(kv_type):
         rows.append(_step(r, prompt[8:], 8, V))
         rows.append(r.executor.launches_per_run())
     assert np.array_equal(rows[0], rows[2]) and rows[1] == rows[3]
+
+
+def test_the_type_is_that_of_the_cache_that_is_held():
+    """A runner that goes from f16 to 4 bits and back computes what fresh runners of each type do."""
+    from ggmlc_b200.runner import load
+
+    gold = np.load(GOLDEN / f"{MODEL}.npz")
+    V, prompt = gold["full_logits"].shape[1], [int(t) for t in gold["prompt"]]
+    fresh = {}
+    for kv_type in ("f16", "q4_0"):
+        r = load(str(GOLDEN / f"{MODEL}.gguf"), device="cuda")
+        r.init_kv_cache(64, kv_type)
+        fresh[kv_type] = _step(r, prompt, 0, V)
+    assert not np.array_equal(fresh["f16"], fresh["q4_0"])
+    r = load(str(GOLDEN / f"{MODEL}.gguf"), device="cuda")
+    assert r.executor.kv_cache_type() == "f16"
+    r.executor.set_kv_cache_type("q4_0")
+    assert r.executor.kv_cache_type() == "q4_0"  # nothing is held yet
+    r.executor.set_kv_cache_type("f16")
+    r.init_kv_cache(64)
+    for kv_type, before in (("q4_0", "f16"), ("f16", "q4_0"), ("q4_0", "f16")):
+        r.executor.set_kv_cache_type(kv_type)
+        assert r.executor.kv_cache_type() == before
+        r.init_kv_cache(64, kv_type)
+        assert r.executor.kv_cache_type() == kv_type
+        assert np.array_equal(_step(r, prompt, 0, V), fresh[kv_type])
+        r.init_kv_cache(64, kv_type)  # the same type: kept, with what it holds
+        assert r.executor.has_kv_cache()
+
+
+def test_the_type_of_a_paged_cache():
+    """init_kv_cache does not replace a paged cache by a contiguous one of another type, and a pool that
+    set_tokens_per_page lays out again keeps its type."""
+    _, ex = _executor()
+    ex.set_tokens_per_page(16)
+    ex.init_paged_kv_cache(2, 64)
+    ex.set_kv_cache_type("q4_0")
+    with pytest.raises(RuntimeError, match="paged"):
+        ex.init_kv_cache(64)
+    ex.set_tokens_per_page(32)
+    assert ex.is_paged_kv_cache_enabled() and ex.kv_cache_type() == "f16"
+    ex.init_paged_kv_cache(2, 64)
+    assert ex.kv_cache_type() == "q4_0"
+    ex.init_kv_cache(64)  # the type that is held: nothing to do, as ever
+    assert ex.is_paged_kv_cache_enabled()
