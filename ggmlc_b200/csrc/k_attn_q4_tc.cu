@@ -95,9 +95,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* b, uint32_t parity) {
         : "memory");
     return done != 0;
 }
-// bounded wait; false (and the CTA's abort flag set) when it runs out.  The test itself may suspend
-// the warp for the hinted time, so a waiting warp leaves the issue slots to the others
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
+// bounded wait of a lane; false (and the CTA's abort flag set) when it runs out.  The test itself may
+// suspend the warp for the hinted time, so a waiting warp leaves the issue slots to the others
+__device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
     if (mbar_test(b, parity)) return true;
     const long long t0 = clock64();
     while (true) {
@@ -116,6 +116,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile
             return false;
         }
     }
+}
+// the same for a warp, whose lanes go on together or give up together: a lane that gave up alone would
+// leave the others at their next vote
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, lane_wait(b, parity, abort));
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -407,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             fetch(0, id, x);
             id = id_of(key(1));
 #pragma unroll 1
-            for (int j = 0; j < steps && !*abort; ++j) {
-                if (!__all_sync(0xffffffffu, decode(j, x)) || j + 1 == steps) break;
+            for (int j = 0; j < steps; ++j) {
+                if (!decode(j, x) || j + 1 == steps) break;
                 fetch(j + 1, id, x);
                 id = id_of(key(j + 2));
             }
@@ -558,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                          : "=r"(elected));
             const bool me = elected != 0;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
-                const bool done = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+                const bool done = mbar_wait(bar, parity, abort);
                 tc_fence_after();
                 return done;
             };
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int row = row0 + tid;
         bool ok = true;
-        if (half && tiles[t] > 0) ok = __all_sync(0xffffffffu, mbar_wait(&q_full[t], 0, abort));  // s_qs
+        if (half && tiles[t] > 0) ok = mbar_wait(&q_full[t], 0, abort);  // s_qs
         const float qs = tiles[t] > 0 ? s_qs[tid] : 0.0f;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 tensor-memory lanes
         const uint32_t ts = tS(t) + lanes, to = tO(t) + lanes;
@@ -729,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // halves of the key tiles in turn: while one is worked on here, the products of the other run
         for (int step = 0; step < 2 * tiles[t] && ok; ++step) {
             const int j = step >> 1, h = step & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t][h], j & 1, abort));
+            ok = mbar_wait(&s_full[t][h], j & 1, abort);
             if (!ok) break;
             tc_fence_after();
             const uint32_t tp = ts + h * kHalf;
@@ -775,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   : j + 1 < tiles[t] ? &s_full[t][0]
                                                      : &o_most[t];
                 const uint32_t parity = h == 0 ? j & 1 : j + 1 < tiles[t] ? (j + 1) & 1 : 0;
-                if (!__all_sync(0xffffffffu, mbar_wait(still, parity, abort))) return false;
+                if (!mbar_wait(still, parity, abort)) return false;
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
@@ -848,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // share TPCs (measured at 333 tokens at 1999: 76 us instead of 73)
         pdl_launch();
         if (ok && tiles[t] > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, abort));
+            ok = mbar_wait(&o_full[t], 0, abort);
             tc_fence_after();
         }
         if (ok) {
