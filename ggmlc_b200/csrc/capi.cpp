@@ -858,6 +858,10 @@ int gb_kv_q4_error(void) {
     const int rc = guard([&] { v = gb::attn_q4_tc_error(); });
     return rc == 0 ? v : -1;
 }
+int gb_kv_q4_clear_error(void) {
+    return guard([&] { gb::attn_q4_tc_clear_error(); });
+}
+void gb_kv_q4_expire_waits(int on) { gb::attn_q4_tc_expire_waits(on != 0); }
 int gb_kv_q4_attend(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, const void* q,
                     int64_t q_row_stride, int64_t q_head_stride, int64_t Hq, int64_t max_kv,
                     float scale, void* o, void* work, size_t work_bytes, void* stream) {

@@ -234,6 +234,12 @@ int Executor::tp_allreduce_error() {
 // A peer all-reduce whose wait ran out wrote a sum that is not valid: every output read of this
 // executor syncs through here and raises (once; the word is cleared) instead of handing it out.
 void Executor::check_tp_error() {
+    if (kv_q4_err_host_ && *(volatile int*)kv_q4_err_host_) {
+        *(volatile int*)kv_q4_err_host_ = 0;
+        throw std::runtime_error(
+            "attention over the 4-bit KV cache: a wait ran out (about 2 s); the outputs of this run are "
+            "not valid");
+    }
     if (chain_err_host_ && *(volatile int*)chain_err_host_) {
         *(volatile int*)chain_err_host_ = 0;
         throw std::runtime_error(
@@ -259,6 +265,7 @@ Executor::~Executor() {
         cudaFree(c.v);
     }
     if (kv_q4_work_) cudaFree(kv_q4_work_);
+    if (kv_q4_err_host_) cudaFreeHost(kv_q4_err_host_);
     for (auto& [id, p] : state_dev_) cudaFree(p);
     for (auto& [k, t] : rope_tabs_) cudaFree(t.first);
     for (cudaEvent_t ev : kevents_) cudaEventDestroy(ev);
@@ -513,6 +520,11 @@ void Executor::alloc_kv_pools(std::map<uint32_t, KVCache>& caches, int64_t slots
             for (auto& [i2, c2] : caches) work = std::max(work, attn_q4_workspace(c2.hd, true));
             GB_CUDA(cudaMalloc(&kv_q4_work_, work));
             GB_CUDA(cudaMemset(kv_q4_work_, 0, work));
+            if (!kv_q4_err_host_) {
+                GB_CUDA(cudaHostAlloc((void**)&kv_q4_err_host_, sizeof(int), cudaHostAllocMapped));
+                *kv_q4_err_host_ = 0;
+                GB_CUDA(cudaHostGetDevicePointer((void**)&kv_q4_err_dev_, kv_q4_err_host_, 0));
+            }
         }
     }
     if (paged) {
@@ -1730,6 +1742,7 @@ std::shared_ptr<Program> Executor::build(const SymEnv& env, bool kv) {
                     qa.max_kv = kv_max_ctx_;
                     qa.scale = scale;
                     qa.work = kv_q4_work_;
+                    qa.err = kv_q4_err_dev_;
                     qa.fast_f32 = true;
                     sb = 0;
                 }

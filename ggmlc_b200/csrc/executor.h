@@ -305,6 +305,8 @@ private:
     bool kv_enabled_ = false;
     int kv_type_want_ = T_F16, kv_type_ = T_F16;  // of the next layout, of the one that is held
     void* kv_q4_work_ = nullptr;  // split scratch of 4-bit cache attention (its counters zeroed once)
+    int* kv_q4_err_host_ = nullptr;  // mapped host memory: a wait of that attention ran out
+    int* kv_q4_err_dev_ = nullptr;
     int64_t kv_max_ctx_ = 0;
     bool paged_ = false;
     int64_t paged_max_batch_ = 0;

@@ -38,7 +38,8 @@
 // (2500 clocks to set up, Q and the first decode 7000) and the output.
 // The loops of the five roles have to fit the instruction cache together; where they did not, both SMs
 // of a TPC ran a quarter slower at times.
-// Every wait is bounded: one that runs out sets the error word and the CTA leaves without output.
+// Every wait is bounded, and a warp's lanes give up together: one that runs out sets the error words,
+// and the rows that depend on it (or their parts, and with them the join) come out NaN.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -69,6 +70,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr long long kSpinCycles = 4000000000LL;  // about 2 s at 1.9 GHz
 
 __device__ int attn_q4_tc_error_word;
+std::atomic<bool> expire_waits{false};
 
 template <int HD, bool K2>
 struct Tc {
@@ -112,7 +114,6 @@ __device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile
         if (*abort) return false;
         if (clock64() - t0 > kSpinCycles) {
             *abort = 1;
-            atomicExch(&attn_q4_tc_error_word, 1);
             return false;
         }
     }
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (tid < NB) s_bad[tid] = INT_MAX;
     if (tid == 0) {
-        s_abort = 0;
+        s_abort = a.expired;
         for (int i = 0; i < 2; ++i) {
             mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], 1);
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_init(&s_full[i][h], 1);
                 mbar_init(&p_full[i][h], 4);
             }
-            mbar_init(&q_full[i], block_rows == kRows ? 8 : 4);
+            mbar_init(&q_full[i], (block_rows == kRows ? 8 : 4) + a.expired);  // (nobody's arrival)
             mbar_init(&o_most[i], 1);
             mbar_init(&o_full[i], 1);
         }
@@ -637,10 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const long long c0 = clock64();
             bool done = false;
             while (!done && clock64() - c0 < kSpinCycles) done = mbar_test(&all_done, 0);
-            if (!done) {
-                *abort = 1;
-                atomicExch(&attn_q4_tc_error_word, 2);
-            }
+            if (!done) *abort = 1;
         }
         __syncwarp();
     } else {
@@ -856,8 +854,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = mbar_wait(&o_full[t], 0, abort);
             tc_fence_after();
         }
-        if (ok) {
-            const float r = alone ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+        {
+            float r = alone ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+            if (l == 0.0f) m = -INFINITY;  // (of a row without keys in this run)
+            if (!ok) r = m = l = __int_as_float(0x7FFFFFFF);
             const uint32_t i_o = (uint32_t)row / (uint32_t)rk, h_o = row - i_o * rk;
             T* op = (T*)a.o + ((int64_t)i_o * a.Hq + hk * rk + h_o) * HD;
             float* part = parts + (((int64_t)(gridDim.x - 1 - blockIdx.x) * a.c.Hkv + hk) * gridDim.z +
@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1  // for the instruction cache, like the masks' few instructions
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t v[32];
-                if (tiles[t] > 0) {
+                if (tiles[t] > 0 && ok) {
                     tmem_ld32(to + c * 32, v);
                     tmem_wait_ld(v);
                 } else {
@@ -894,13 +894,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (row < row1 && !alone)
-                *(float2*)(part + block_rows * HD + tid * 2) =
-                    make_float2(l != 0.0f ? m : -INFINITY, l);
+                *(float2*)(part + block_rows * HD + tid * 2) = make_float2(m, l);
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
+        if (*abort) {
+            attn_q4_tc_error_word = 1;
+            if (a.err) *(volatile int*)a.err = 1;  // mapped host memory
+        }
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
@@ -1010,6 +1013,7 @@ void launch_tc(const AttnQ4Args& a, cudaStream_t st) {
     AttnQ4Args b = a;
     b.shift = kv_q4_shift(a.c);
     b.q_vec = kv_q4_vectors(a);
+    b.expired = expire_waits;
     float* parts = (float*)((char*)a.work + attn_q4_parts_offset());
     launch_pdl(k_attn_q4_tc<T, HD, TWO>, dim3((unsigned)plan.blocks, a.c.Hkv, plan.splits),
                dim3(kThreads), S::kSmem, st, b, plan.block_rows, parts);
@@ -1051,6 +1055,13 @@ void launch_attn_q4_tc(const AttnQ4Args& a, cudaStream_t st) {
     else
         launch_tc_hd<__nv_bfloat16, false>(a, st);
     GB_CUDA(cudaGetLastError());
+}
+
+void attn_q4_tc_expire_waits(bool on) { expire_waits = on; }
+
+void attn_q4_tc_clear_error() {
+    const int v = 0;
+    GB_CUDA(cudaMemcpyToSymbol(attn_q4_tc_error_word, &v, sizeof v));
 }
 
 int attn_q4_tc_error() {

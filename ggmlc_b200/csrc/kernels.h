@@ -446,6 +446,8 @@ struct AttnQ4Args {
     // f16, the probabilities in two terms (the engine's prefill; its attention over an f16 cache rounds
     // q and the probabilities to f16 too); otherwise f32 keeps two-term products
     bool fast_f32 = false;
+    int* err = nullptr;  // set to 1 (device-accessible host memory) when a wait of the call runs out
+    bool expired = false;  // set by the launcher: attn_q4_tc_expire_waits
 };
 // q can be read in 16-byte pieces: its base and strides are whole ones
 inline bool kv_q4_vectors(const AttnQ4Args& a) {
@@ -459,11 +461,14 @@ double attn_q4_tc_us(const AttnQ4Args& a);         // the chunk kernel's time, a
 bool attn_q4_head_dim(int64_t hd);  // head dims the attention kernels are built for
 void launch_attn_q4(const AttnQ4Args& a, cudaStream_t st);
 // The same for a chunk (pos and slot NULL) on tcgen05 (k_attn_q4_tc.cu): f16 / bf16 q, f32 with
-// fast_f32, head_dim 64 or 128; launch_attn_q4 sends the chunks there that fill its tiles.  attn_q4_tc_error: its sticky
-// error word (non-zero after one of its bounded waits ran out).
+// fast_f32, head_dim 64 or 128; launch_attn_q4 sends the chunks there that fill its tiles.  A wait of
+// its that runs out makes the rows NaN and sets *err and the sticky error word , attn_q4_tc_error;
+// attn_q4_tc_expire_waits: in later launches one wait has no end and all count as run out.
 bool attn_q4_tc_fits(const AttnQ4Args& a);
 void launch_attn_q4_tc(const AttnQ4Args& a, cudaStream_t st);
 int attn_q4_tc_error();
+void attn_q4_tc_clear_error();
+void attn_q4_tc_expire_waits(bool on);
 
 // ---- decode chain (k_chain.cu) ---------------------------------------------------------------
 // The launches of one single-sequence decode step — quantized GEMVs with their RMSNorm / quantize

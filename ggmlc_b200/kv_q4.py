@@ -51,7 +51,10 @@ for _name, _args, _res in (
         ("gb_kv_q4_attend_workspace_bytes", [_P, _I64, _I64], _SZ),
         ("gb_kv_q4_attend", [_P, _P, _I, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ, _P], _I),
         ("gb_kv_q4_attend_prefill", [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ,
-                                     _P], _I)):
+                                     _P], _I),
+        ("gb_kv_q4_error", [], _I),
+        ("gb_kv_q4_clear_error", [], _I),
+        ("gb_kv_q4_expire_waits", [_I], None)):
     getattr(_lib, _name).argtypes = _args
     getattr(_lib, _name).restype = _res
 
@@ -62,6 +65,22 @@ def page_bytes(page_len: int, head_dim: int) -> int:
     if n < 0:
         raise ValueError("page_len must be a positive multiple of 16 and head_dim of 32")
     return n
+
+
+def error() -> int:
+    """Non-zero once a bounded wait inside the attention of a chunk has run out on the current device
+    (after about 2 s; that call's rows are NaN); waits for the device.  ``clear_error()`` resets it."""
+    torch.cuda.synchronize()
+    v = int(_lib.gb_kv_q4_error())
+    if v < 0:
+        raise RuntimeError(_lib.gb_last_error().decode())
+    return v
+
+
+def clear_error() -> None:
+    torch.cuda.synchronize()
+    if _lib.gb_kv_q4_clear_error() != 0:
+        raise RuntimeError(_lib.gb_last_error().decode())
 
 
 class Q4KVCache(_kv_q4.Cache):

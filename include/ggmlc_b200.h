@@ -449,8 +449,13 @@ int gb_kv_q4_attend_prefill(const gb_kv_q4* cache, int64_t n_rows, const int64_t
                             int64_t q_head_stride, int64_t Hq, int64_t max_kv, float scale, float* o,
                             void* work, size_t work_bytes, void* stream);
 /* Sticky error word of the chunk kernel: 0 while every bounded wait in it completed, non-zero after
- * one ran out (that call's output is not valid), -1 if the word cannot be read. */
+ * one ran out (the rows concerned are NaN), -1 if the word cannot be read.  An executor raises such an
+ * error by itself when its outputs are read. */
 int gb_kv_q4_error(void);
+int gb_kv_q4_clear_error(void);
+/* For tests of all that: in later chunk calls one wait is for nothing, and every wait that does not
+ * end at once counts as run out. */
+void gb_kv_q4_expire_waits(int on);
 
 #ifdef __cplusplus
 }

@@ -306,3 +306,43 @@ def test_prefill_form_refusals():
     refused("head_dim", cache=wide)
     refused("work", work=None)
     refused("work", work=p + 16)
+
+
+# ---- a wait that runs out ----------------------------------------------------------------------------
+@pytest.fixture
+def no_waiting():
+    """Waits inside the chunk kernel count as run out."""
+    torch = _torch()
+    assert kv_q4.error() == 0  # of all calls before, in whatever test
+    kv_q4._lib.gb_kv_q4_expire_waits(1)
+    try:
+        yield
+    finally:
+        kv_q4._lib.gb_kv_q4_expire_waits(0)
+        torch.cuda.synchronize()
+        kv_q4.clear_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("s, past", [(512, 0), (200, 3000)])  # whole blocks; runs of key tiles and a join
+def test_a_wait_that_runs_out_shows(no_waiting, dtype, s, past):
+    """Rows come out NaN, never stale, the error word is set, and the next call is as ever."""
+    torch = _torch()
+    cache = make_cache(torch, 1, -(-(past + s) // 64), 8, 64, 128, True, 71)
+    held = fill(torch, cache, [past + s], 72)
+    q = torch.randn(s, 32, 128, generator=torch.Generator().manual_seed(73))
+    q = q.to(getattr(torch, dtype)).cuda()
+    want, tol = expect(torch, q, held, range(past, past + s), [0] * s, 1 / math.sqrt(128))
+    kv_q4._lib.gb_kv_q4_expire_waits(0)
+    check(torch, cache.attend(q, past, 0), want, tol)  # leaves good partials in the scratch
+    assert kv_q4.error() == 0
+    kv_q4._lib.gb_kv_q4_expire_waits(1)
+    out = torch.zeros_like(q)
+    cache.attend(q, past, 0, out=out)
+    assert kv_q4.error() != 0
+    assert out.isnan().all()
+    kv_q4._lib.gb_kv_q4_expire_waits(0)
+    kv_q4.clear_error()
+    check(torch, cache.attend(q, past, 0), want, tol)
+    assert kv_q4.error() == 0

@@ -50,3 +50,24 @@ def test_long_prompts_follow_the_oracle(model, window, chunk, graph):
     assert min(cos(a, b) for a, b in zip(got[::37], rows[::37])) >= COS_MIN - 0.002
     token = int(rows[-1].argmax())
     assert cos(_step(r, [token], TOKENS, VOCAB), step) >= COS_MIN
+
+
+def test_a_wait_that_runs_out_is_raised(model):
+    """Reading the outputs of a prefill whose attention gave up raises once; the next prefill is as
+    ever."""
+    from ggmlc_b200 import kv_q4
+    from ggmlc_b200.runner import load
+
+    path, prompt, rows, _ = model
+    r = load(str(path), device="cuda")
+    r.executor.set_enable_cuda_graph(False)
+    r.init_kv_cache(512, "q4_0")
+    try:
+        kv_q4._lib.gb_kv_q4_expire_waits(1)
+        with pytest.raises(RuntimeError, match="4-bit KV cache"):
+            _step(r, prompt, 0, VOCAB)
+    finally:
+        kv_q4._lib.gb_kv_q4_expire_waits(0)
+        kv_q4.clear_error()
+    assert cos(_step(r, prompt, 0, VOCAB), rows) >= COS_MIN
+    assert kv_q4.error() == 0
