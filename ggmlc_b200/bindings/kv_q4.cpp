@@ -72,6 +72,15 @@ class Cache {
             c_.n_slots = pages_->size(0);
             c_.pages_per_slot = pages_->size(1);
         }
+        if (shared().handles++ == 0) shared().work = new ScratchMap;
+    }
+    Cache(const Cache&) = delete;
+    Cache& operator=(const Cache&) = delete;
+    ~Cache() {
+        if (--shared().handles == 0) {
+            delete shared().work;
+            shared().work = nullptr;
+        }
     }
 
     void write(const at::Tensor& k, const at::Tensor& v, const py::object& pos,
@@ -118,8 +127,9 @@ class Cache {
             o = at::detail::empty_cuda(q.sizes(), q.scalar_type(), k_.device(), std::nullopt);
         }
         const cudaStream_t st = stream();
-        const size_t need = gb_kv_q4_attend_workspace_bytes(&c_, n, q.size(1));
-        const at::Tensor& work = scratch(st, (int64_t)need);
+        const size_t need =
+            gb_kv_q4_attend_workspace_bytes(&c_, r.pos || r.slot ? std::min<int64_t>(n, 1) : n, q.size(1));
+        const at::Tensor& work = scratch(k_.device(), st, (int64_t)need);
         check(gb_kv_q4_attend(&c_, &r, type_id(q.scalar_type()), q.data_ptr(), q.stride(0),
                               q.stride(1), q.size(1), max_kv,
                               (float)scale.value_or(1.0 / std::sqrt((double)c_.head_dim)),
@@ -140,21 +150,22 @@ class Cache {
         return c10::cuda::getCurrentCUDAStream(k_.device().index()).stream();
     }
 
-    // Split scratch, one per stream: its calls run one after the other.  A call under capture never
+    // Split scratch, one per device and stream for all handles: calls on a stream run one after the
+    // other (a handle a layer would hold 1.2 GB for 32 layers).  A call under capture never
     // gets the memory of eager calls, which a larger call replaces, nor another capture's, which may
     // replay at the same time or before it: each capture has its own, from the graph's pool, whose
     // counters its first call zeroes as a node of that graph.  The pool keeps it for as long as the
     // graph lives, also after the next capture on the stream has taken its place here.
-    const at::Tensor& scratch(cudaStream_t st, int64_t need) {
+    static const at::Tensor& scratch(at::Device device, cudaStream_t st, int64_t need) {
         cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
         unsigned long long id = 0;
         if (cudaStreamGetCaptureInfo(st, &status, &id) != cudaSuccess)
             throw std::runtime_error("Q4KVCache: the stream's capture status cannot be read");
-        Scratch& s = work_[st];
+        Scratch& s = (*shared().work)[{device.index(), st}];
         const bool capturing = status == cudaStreamCaptureStatusActive;
         at::Tensor& work = capturing ? s.captured : s.eager;
         if (!work.defined() || work.numel() < need || (capturing && s.capture != id)) {
-            work = at::empty({need}, k_.options());
+            work = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(device));
             // the counters are zero before the first call and after every one
             work.narrow(0, 0, std::min<int64_t>(need, GB_KV_Q4_WORK_ZEROED)).zero_();
             if (capturing) s.capture = id;
@@ -216,7 +227,16 @@ class Cache {
         at::Tensor eager, captured;
         unsigned long long capture = 0;  // the capture `captured` belongs to
     };
-    std::map<cudaStream_t, Scratch> work_;
+    using ScratchMap = std::map<std::pair<int, cudaStream_t>, Scratch>;
+    // of the process, freed with its last handle; under the interpreter's lock, like every call here
+    struct Shared {
+        int handles = 0;
+        ScratchMap* work = nullptr;
+    };
+    static Shared& shared() {
+        static Shared s;
+        return s;
+    }
 };
 
 }  // namespace

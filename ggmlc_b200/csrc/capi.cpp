@@ -109,7 +109,8 @@ gb::AttnQ4Args attn_q4_of(const gb_kv_q4* cache, const gb_kv_rows* rows, int typ
     if (a.r.n == 0) return a;
     GB_CHECK(q && o, what + ": q and o must not be NULL");
     GB_CHECK(work && ((uintptr_t)work & 255) == 0 &&
-                 work_bytes >= gb::attn_q4_workspace(a.c.hd, a.r.n > 1),
+                 work_bytes >=
+                     gb::attn_q4_workspace(a.c.hd, a.r.n > 1 && !a.r.pos && !a.r.slot),
              what + ": work must be gb_kv_q4_attend_workspace_bytes() of 256-byte aligned device "
                     "memory");
     a.type = type;

@@ -199,7 +199,7 @@ struct Segment {
 };
 
 // CTAs of one launch: the machine filled once.  The workspace: 3 counters per CTA, then 4 partials
-constexpr int kMaxCtas = 1024, kMaxCtasPerSm = 4;
+constexpr int kMaxCtas = 1024, kMaxCtasPerSm = 3;
 constexpr int64_t kCounterBytes = 3 * kMaxCtas * 4;
 static_assert(kCounterBytes <= GB_KV_Q4_WORK_ZEROED, "the counters are what callers zero");
 constexpr int64_t partial_floats(int64_t hd) { return kHeads * (hd + 2); }

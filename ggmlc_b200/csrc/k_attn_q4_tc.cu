@@ -1033,15 +1033,19 @@ void launch_tc_hd(const AttnQ4Args& a, cudaStream_t st) {
 
 }  // namespace
 
+bool tc_head_dim(int64_t hd) { return hd == 64 || hd == 128; }
+
 // bytes of the partials behind attn_q4_parts_offset(): at most two CTAs an SM leave one
-size_t attn_q4_tc_parts(int64_t hd) { return (size_t)(2 * current_sms() * part_floats(2 * kRows, hd) * 4); }
+size_t attn_q4_tc_parts(int64_t hd) {
+    return tc_head_dim(hd) ? (size_t)(2 * current_sms() * part_floats(2 * kRows, hd) * 4) : 0;
+}
 
 double attn_q4_tc_us(const AttnQ4Args& a) {
     return tc_plan(a.r.n, a.Hq / a.c.Hkv, a.c.Hkv, keys_of(a), current_sms()).us;
 }
 
 bool attn_q4_tc_fits(const AttnQ4Args& a) {
-    return !a.r.pos && !a.r.slot && (a.c.hd == 64 || a.c.hd == 128) &&
+    return !a.r.pos && !a.r.slot && tc_head_dim(a.c.hd) &&
            a.r.n * (a.Hq / a.c.Hkv) < (int64_t(1) << 30) &&
            (a.type == kTypeF16 || a.type == kTypeBF16 || (a.type == kTypeF32 && a.fast_f32)) &&
            ((uintptr_t)a.o & 15) == 0;

@@ -454,15 +454,16 @@ inline bool kv_q4_vectors(const AttnQ4Args& a) {
     const int64_t es = a.type == kTypeF32 ? 4 : 2;
     return ((uintptr_t)a.q & 15) == 0 && (a.q_row * es) % 16 == 0 && (a.q_head * es) % 16 == 0;
 }
-size_t attn_q4_workspace(int64_t hd, bool chunks);  // chunks: calls of consecutive rows among them
+// bytes of work for calls of one head_dim; chunks: those of several consecutive rows among them
+size_t attn_q4_workspace(int64_t hd, bool chunks);
 size_t attn_q4_parts_offset();                     // partials start behind the counters
-size_t attn_q4_tc_parts(int64_t hd);
+size_t attn_q4_tc_parts(int64_t hd);               // 0 for head dims that kernel is not built for
 double attn_q4_tc_us(const AttnQ4Args& a);         // the chunk kernel's time, as its launch plans it
 bool attn_q4_head_dim(int64_t hd);  // head dims the attention kernels are built for
 void launch_attn_q4(const AttnQ4Args& a, cudaStream_t st);
 // The same for a chunk (pos and slot NULL) on tcgen05 (k_attn_q4_tc.cu): f16 / bf16 q, f32 with
 // fast_f32, head_dim 64 or 128; launch_attn_q4 sends the chunks there that fill its tiles.  A wait of
-// its that runs out makes the rows NaN and sets *err and the sticky error word , attn_q4_tc_error;
+// its that runs out makes the rows NaN and sets *err and the sticky error word, attn_q4_tc_error;
 // attn_q4_tc_expire_waits: in later launches one wait has no end and all count as run out.
 bool attn_q4_tc_fits(const AttnQ4Args& a);
 void launch_attn_q4_tc(const AttnQ4Args& a, cudaStream_t st);

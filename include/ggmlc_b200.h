@@ -435,6 +435,7 @@ int gb_kv_q4_read(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, void*
  * call leaves them zero); calls that can overlap, replays of captured graphs among them, need one
  * each, and memory that a graph has captured has to outlive it. */
 #define GB_KV_Q4_WORK_ZEROED 16384
+/* n_rows: the most consecutive rows of one call; 1 where pos or slot is an array, whatever n is. */
 size_t gb_kv_q4_attend_workspace_bytes(const gb_kv_q4* cache, int64_t n_rows, int64_t Hq);
 int gb_kv_q4_attend(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, const void* q,
                     int64_t q_row_stride, int64_t q_head_stride, int64_t Hq, int64_t max_kv,

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import gc
 import math
 import re
 from pathlib import Path
@@ -346,3 +347,59 @@ def test_a_wait_that_runs_out_shows(no_waiting, dtype, s, past):
     kv_q4.clear_error()
     check(torch, cache.attend(q, past, 0), want, tol)
     assert kv_q4.error() == 0
+
+
+# ---- scratch -------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_handles_share_the_scratch_of_a_stream():
+    """A handle a layer, chunks and single rows: no more scratch than one handle holds; none is left
+    when the handles are gone."""
+    torch = _torch()
+    gc.collect()
+    none = torch.cuda.memory_allocated()
+    caches = [make_cache(torch, 1, 40, 8, 64, 128, True, 81 + i) for i in range(8)]
+    held = [fill(torch, c, [2500], 90 + i) for i, c in enumerate(caches)]
+    q = torch.randn(100, 32, 128, device="cuda").bfloat16()
+    before = torch.cuda.memory_allocated()
+    outs = [caches[0].attend(q, 2400, 0)]
+    one = torch.cuda.memory_allocated() - before
+    assert 0 < one < 48 << 20
+    outs += [c.attend(q, 2400, 0) for c in caches[1:]]
+    rows = [c.attend(q[:1], 2399, 0) for c in caches]
+    assert torch.cuda.memory_allocated() - before < one + 17 * outs[0].numel() * 2
+    for h, o, r in zip(held, outs, rows):
+        check(torch, o, *expect(torch, q, h, range(2400, 2500), [0] * 100, 1 / math.sqrt(128)))
+        check(torch, r, *expect(torch, q[:1], h, [2399], [0], 1 / math.sqrt(128)))
+    del caches, held, q, outs, rows, h, o, r
+    gc.collect()
+    assert torch.cuda.memory_allocated() <= none + 64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_scratch_is_what_a_call_can_use(hd):
+    """Single rows, calls with a position or slot each, and head_dim 256 never reach the tiles."""
+    torch = _torch()
+    c = _c_cache(kv_q4, head_dim=hd)
+    need = lambda n: kv_q4._lib.gb_kv_q4_attend_workspace_bytes(ctypes.addressof(c), n, 4)
+    assert (need(2) > need(1)) == (hd < 256) and need(1) < 20 << 20
+    cache = make_cache(torch, 2, 8, 2, 64, hd, True, 95)
+    held = fill(torch, cache, [500, 300], 96)
+    q = torch.randn(2, 4, hd, device="cuda")
+    pos = torch.tensor([499, 299], dtype=torch.int32, device="cuda")
+    slot = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    work = torch.zeros(need(1), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    c = kv_q4._Cache(cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0], 64, 2, hd,
+                     cache.pages.data_ptr(), *cache.pages.shape)
+    r = kv_q4._Rows(2, pos.data_ptr(), 0, slot.data_ptr(), 0)
+
+    def call(size):
+        return kv_q4._lib.gb_kv_q4_attend(
+            ctypes.addressof(c), ctypes.addressof(r), 0, q.data_ptr(), q.stride(0), q.stride(1), 4, 0,
+            1 / math.sqrt(hd), out.data_ptr(), work.data_ptr(), size,
+            torch.cuda.current_stream().cuda_stream)
+
+    assert call(need(1) - 1) == -1 and "work" in kv_q4._lib.gb_last_error().decode()
+    assert call(need(1)) == 0
+    check(torch, out, *expect(torch, q, held, [499, 299], [0, 1], 1 / math.sqrt(hd)))
