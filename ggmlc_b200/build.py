@@ -4,12 +4,14 @@
 
 Objects go to ggmlc_b200/_build/; a source is recompiled when it or any header in csrc/ is
 newer than its object.  The shared library links the CUDA runtime statically so it loads in
-any process of this image (with or without torch).
+any process of this image (with or without torch).  Where torch is installed, the binding of the
+4-bit KV cache operators (_kv_q4.so) is built against it as well.
 """
 
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -99,14 +101,36 @@ def build_bench_tool(force: bool = False) -> Path:
 
 BINDING_SRC = PKG / "bindings" / "kv_q4.cpp"
 BINDING = PKG / "_kv_q4.so"
+BINDING_FOR = BUILD / "_kv_q4.for"  # what it was built against
 
 
-def build_torch_binding(force: bool = False) -> Path:
+def torch_build() -> str | None:
+    """What the torch binding is compiled against (interpreter, torch and its ABI), None where torch
+    with its C++ headers and CUDA is not installed.  Found without importing torch, which takes seconds."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return None
+    root = Path(list(spec.submodule_search_locations)[0])
+    needs = ("include/torch/csrc/utils/pybind.h", "lib/libc10_cuda.so", "lib/libtorch_python.so")
+    if not all((root / f).exists() for f in needs):
+        return None
+    version = root / "version.py"
+    tag = version.read_text() if version.exists() else ""
+    return "\n".join([sys.version, str(root), tag])
+
+
+def build_torch_binding(force: bool = False) -> Path | None:
     """ggmlc_b200/_kv_q4.so: the torch binding of the 4-bit KV cache operators (host C++ against
-    torch's headers and the library above)."""
+    torch's headers and the library above), built anew when the source, the header, torch or the
+    interpreter changes.  None where there is no torch to build it against: only ggmlc_b200.kv_q4
+    needs it, the engine does not."""
+    against = torch_build()
+    if against is None:
+        return None
     header = PKG.parent / "include" / "ggmlc_b200.h"
     if not force and BINDING.exists() and BINDING.stat().st_mtime >= max(
-            BINDING_SRC.stat().st_mtime, header.stat().st_mtime):
+            BINDING_SRC.stat().st_mtime, header.stat().st_mtime) and (
+            BINDING_FOR.exists() and BINDING_FOR.read_text() == against):
         return BINDING
     import sysconfig
 
@@ -130,6 +154,8 @@ def build_torch_binding(force: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"torch binding build failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDING)
+    BUILD.mkdir(exist_ok=True)
+    BINDING_FOR.write_text(against)
     return BINDING
 
 
