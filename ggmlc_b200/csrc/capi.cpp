@@ -106,6 +106,7 @@ gb::AttnQ4Args attn_q4_of(const gb_kv_q4* cache, const gb_kv_rows* rows, int typ
     GB_CHECK(Hq > 0 && Hq <= 65536 && Hq % a.c.Hkv == 0,
              what + ": Hq must be a multiple of n_kv_heads");
     GB_CHECK(q_row >= 0 && q_head >= 0, what + ": strides must not be negative");
+    GB_CHECK(std::isfinite(scale), what + ": scale must be finite");
     if (a.r.n == 0) return a;
     GB_CHECK(q && o, what + ": q and o must not be NULL");
     GB_CHECK(work && ((uintptr_t)work & 255) == 0 &&

@@ -426,7 +426,7 @@ int gb_kv_q4_read(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, void*
 /* Attention of q rows [n][Hq][head_dim] (strides in elements, dims contiguous) over the cache, GQA
  * (Hq a multiple of n_kv_heads): row r sees positions 0 .. min(pos, max_kv - 1) of its sequence,
  * max_kv <= 0: the sequence's whole capacity; a row that sees none (position -1) gets zeros.
- * Positions on a page outside the pool are not seen.  Values past a row's positions may be
+ * scale: finite.  Positions on a page outside the pool are not seen.  Values past a row's positions may be
  * anything (NaN included), also where other rows of the call see them.  A seen value whose scale
  * is beyond 8188 in magnitude, which no write stores, may count as NaN.  o: contiguous [n][Hq][head_dim] of q's type.  head_dim 64, 128 or 256.
  * Arithmetic: f32 q to about 1e-6 of fp32 (two-term f16 products, fp32 sums); f16 / bf16 q: V and

@@ -403,3 +403,17 @@ def test_scratch_is_what_a_call_can_use(hd):
     assert call(need(1) - 1) == -1 and "work" in kv_q4._lib.gb_last_error().decode()
     assert call(need(1)) == 0
     check(torch, out, *expect(torch, q, held, [499, 299], [0, 1], 1 / math.sqrt(hd)))
+
+
+# ---- refusals ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_a_scale_that_is_no_number_is_refused(scale):
+    """(It came out as a scale too small to tell scores apart: the mean of V.)"""
+    c, p, L = _c_cache(kv_q4), 1 << 23, kv_q4._lib
+    r = kv_q4._Rows(1, None, 0, None, 0)
+    assert L.gb_kv_q4_attend(ctypes.addressof(c), ctypes.addressof(r), 0, p, 128, 64, 2, 0, scale, p, p,
+                             1 << 30, None) == -1
+    assert "scale" in L.gb_last_error().decode()
+    assert L.gb_kv_q4_attend_prefill(ctypes.addressof(c), 1, p, 0, p, 128, 64, 2, 0, scale, p, p, 1 << 30,
+                                     None) == -1
+    assert "scale" in L.gb_last_error().decode()
