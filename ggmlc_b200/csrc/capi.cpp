@@ -74,8 +74,9 @@ gb::KvQ4 kv_q4_of(const gb_kv_q4* c, const std::string& what) {
     r.n_slots = c->pages ? c->n_slots : c->n_pages;
     r.per_slot = c->pages ? c->pages_per_slot : 1;
     GB_CHECK(r.n_slots > 0 && r.per_slot > 0, what + ": the page table must not be empty");
-    GB_CHECK(r.per_slot <= 0x7FFFFFFF / r.page_len,
-             what + ": a sequence's capacity must stay below 2^31 positions");
+    // the kernels count positions in int, a few tiles of keys past the end too
+    GB_CHECK(r.per_slot <= (0x7FFFFFFF - 4096) / r.page_len,
+             what + ": a sequence's capacity must stay 4096 positions below 2^31");
     return r;
 }
 gb::KvQ4Rows kv_q4_rows_of(const gb_kv_rows* r, const std::string& what) {

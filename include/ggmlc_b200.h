@@ -395,7 +395,8 @@ int gb_attention(const float* q, const void* k, const void* v, int64_t hd, int64
  * equals), d = m / -8, code = min(15, floor(x / d + 8.5)), scale = fp16(d); a scale that rounds to
  * zero stores zeros, a block with a NaN reads back as NaN.
  * pages: int32 [n_slots][pages_per_slot], the pages of each sequence in order, or NULL: page
- * `slot` is the sequence's whole window (n_slots = n_pages, pages_per_slot = 1). */
+ * `slot` is the sequence's whole window (n_slots = n_pages, pages_per_slot = 1).  A sequence holds
+ * less than 2^31 - 4096 positions. */
 typedef struct gb_kv_q4 {
     void* k;
     void* v;

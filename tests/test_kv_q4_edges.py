@@ -417,3 +417,15 @@ def test_a_scale_that_is_no_number_is_refused(scale):
     assert L.gb_kv_q4_attend_prefill(ctypes.addressof(c), 1, p, 0, p, 128, 64, 2, 0, scale, p, p, 1 << 30,
                                      None) == -1
     assert "scale" in L.gb_last_error().decode()
+
+
+@pytest.mark.parametrize("per_slot, ok", [((2**31 - 1) // 64, False), ((2**31 - 4096) // 64 + 1, False),
+                                          ((2**31 - 4097) // 64, True)])
+def test_a_capacity_near_two_to_the_31(per_slot, ok):
+    """Positions are ints in the kernels, and tiles of keys run past a sequence's end: the last 4096
+    below 2^31 are refused (page tables can repeat pages, so no memory stands in the way)."""
+    c, L = _c_cache(kv_q4, pages_per_slot=per_slot), kv_q4._lib
+    none = kv_q4._Rows(0, None, 0, None, 0)  # no rows: nothing is launched
+    rc = L.gb_kv_q4_read(ctypes.addressof(c), ctypes.addressof(none), 0, None, None, None)
+    assert rc == (0 if ok else -1), L.gb_last_error()
+    assert ok or "2^31" in L.gb_last_error().decode()
