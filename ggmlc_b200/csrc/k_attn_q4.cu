@@ -22,12 +22,17 @@
 //   q is multiplied by a power of two per head, the largest element in [1, 2), so that bf16 and
 //      f32 inputs fit f16; the factor returns in the softmax scale.
 //   V: (n - 8) * d in f16, one rounding (16-bit types); f32: that and the exact remainder as a
-//      second f16 term.  Scales of positions past n_r are replaced by zero, and their scores by
+//      second f16 term.  The rounding is 2^-12 of values whose codes are off by up to 2^-4 of their
+//      block's extreme.  For f16 it is what is left above the rounding of the output (error against 64
+//      bits 2.6e-4, the output alone 2.1e-4); the second term costs a row of 131071 positions 64 us
+//      instead of 54.  Scales of positions past n_r are replaced by zero, and their scores by
 //      -inf, by selection: what the memory holds there (NaN included) is never multiplied in.
 //      Packed positions see different numbers of keys: a key that only some of them see and whose
 //      V scale is no number gets scale zero, and the columns that see it get their NaN by addition.
 //   P: exp2(s - m + 14) in f16 (two terms for f32 and f16 outputs); the factor 2^14 cancels in O / l and
-//      keeps small probabilities out of f16's subnormals.
+//      keeps small probabilities out of f16's subnormals.  One term is enough for bf16, whose error is
+//      1.6e-3 as the output's rounding alone makes; two cost 64 ragged rows 164 us instead of 151.
+//      Whoever wants f32's arithmetic for 16-bit data passes q as f32 (227 us).
 //
 // Work split: a step is a run of kKeys keys of one row, KV head and up to 8 heads of its group; a
 // segment is one CTA's run of steps of one row and head group, its 4 warps taking them in turn.
@@ -44,9 +49,9 @@
 // step, or one per 16 keys where a page ends inside a step.  (Bulk copies issued by one lane took
 // 4 per warp and step; their operands cost a fifth of the loop's issue slots.)
 // Bound: by issue slots.  A step of 32 keys at head_dim 128 is 737 warp instructions in bf16 (321 of
-// them integer, 262 fp), at 2.6 a clock and SM: 64 rows of 1..16384 positions of 8 x 128 149 us (the
-// bytes alone 93), one row of 131071 in f16 54 us (23).  Short rows by latency: one of 640 in f32 9.5
-// us, of which an empty launch is 2.2.
+// them integer, 262 fp), at 2.6 a clock and SM: 64 rows of 1..16384 positions of 8 x 128 151 us (the
+// bytes alone 93), one row of 131071 in f16 55 us (23).  Short rows by latency: one of 640 in f32 10.4
+// us, of which an empty launch is 2.2.  (Calls queued one after the other, CUDA events.)
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -360,8 +365,8 @@ __global__ void __launch_bounds__(Shape<HD, PREC>::kWarps * 32, Shape<HD, PREC>:
     if (apart) {
         // The machine filled once, but no CTA for less than kMinSteps, or one step a warp where that
         // leaves the longest row at most kFan parts, which one CTA joins.  Measured, f32: 640 positions
-        // 11.9 us with 8 steps a CTA, 9.5 with 4; 2000 positions 12.5 with 8, 14.6 with 5 and two levels
-        // of joins; 200 positions 8.3 whole, 8.5 with 4.
+        // 11.4 us with 8 steps a CTA, 10.4 with 4 (1000 positions 12.0 and 10.6); 2000 positions 12.5 with
+        // 8, 14.6 with 5 and two levels of joins; 200 positions 9.4 whole, 9.6 with 4.
         const int least = s_longest > kMinSteps && s_longest <= kWarps * kFan ? kWarps : kMinSteps;
         budget = max((long long)least, (steps_all - 1) / ((long long)gridDim.x - rows * hgs) + 1);
         __syncthreads();

@@ -1,5 +1,6 @@
 // Attention of a chunk (consecutive positions of one sequence, causal) over a KV cache held in 4
-// bits, on the 5th-generation tensor cores: f16 and bf16 q, head_dim 64 and 128.
+// bits, on the 5th-generation tensor cores: f16 and bf16 q, and f32 q of the engine's prefill
+// (fast_f32), head_dim 64 and 128.
 //
 // A CTA takes two tiles of 128 q rows of one KV head, a row being a (position, head of the group)
 // pair, and walks the keys in tiles of 128: S = Q K^T and O += P V as tcgen05.mma kind::f16 with
@@ -10,13 +11,17 @@
 // instructions; two tiles let the softmax of one run under the products of the other.
 //   K, V: (code - 8) * scale in f16, one rounding; for f16 calls K as the sum of two f16 terms, which
 //   is exact (Q once more).  Measured at 333 tokens at 1999: 68 -> 83 us, and the error against 64
-//   bits from 3.3e-4 to 2.6e-4 where rounding the output alone makes 2.1e-4.
+//   bits from 3.3e-4 to 2.6e-4 where rounding the output alone makes 2.1e-4.  V's second term has no
+//   room in shared memory beside two tiles of Q (two stages of K and of V and K's second terms fill it).
+//   bf16 calls: 1.68e-3, where rounding the output makes 1.66e-3; with f16's terms 2048 tokens at 14336
+//   take 913 us instead of 565.  The engine's f32: 3.3e-4, of the size of what its prefill over an f16
+//   cache rounds; 512 tokens at 0 take 20 us, with the rows kernel's 22 bits (3e-7) 65.
 //   V of a key that only some rows of the CTA see must not reach the others through 0 x NaN: there a
 //   scale that is no number is decoded as zero, and the first such key of each block of 32 dims kept;
 //   rows that see it get NaN in the block when they are written.
 //   q: f16 after a power of two per row, the largest element in [1, 2) (exact for bf16 but for
 //   elements 2^-14 below it); the factor returns in the softmax scale.
-//   P: exp2(s - m + 7) in f16, for f16 outputs as the sum of two f16 terms (V once more).  m is a
+//   P: exp2(s - m + 7) in f16, for f16 and f32 outputs as the sum of two f16 terms (V once more).  m is a
 //   running maximum that is renewed only when a P would pass 2^15 (f16 holds 2^16): the scores are
 //   read once, and O is rarely rescaled.
 // Operands: all K-major with the 128-byte swizzle.  Q and K rows hold the 8 dims of a word in the
@@ -33,9 +38,10 @@
 //             memory (17-19 idle).
 // Bound: at head_dim 128 a key tile costs 2048 clocks of tensor work (4 products of 128^3 at 4096
 // multiply-adds a clock) and 2048 of exponentials (16 a clock), overlapped.
-// Measured (bf16): 2048 tokens at 14336 of 32 heads 542 us, 951 TFLOP/s, the tensor pipe half busy, a
-// pair of tiles about 3600 clocks a key tile; 512 at 0 15.4 us, of which 7 are the first scores' way
-// (2500 clocks to set up, Q and the first decode 7000) and the output.
+// Measured (bf16): 2048 tokens at 14336 of 32 heads 565 us, 912 TFLOP/s (600 us with other inputs from
+// call to call), the tensor pipe half busy, a pair of tiles about 3700 clocks a key tile; 512 at 0 16
+// us, of which 7 are the first scores' way (2500 clocks to set up, Q and the first decode 7000) and the
+// output.
 // The loops of the five roles have to fit the instruction cache together; where they did not, both SMs
 // of a TPC ran a quarter slower at times.
 // Every wait is bounded, and a warp's lanes give up together: one that runs out sets the error words,
@@ -260,8 +266,9 @@ __device__ __forceinline__ void tmem_wait_st() {
 // f16 makes 2.4e-4).  -inf gives exactly 0; z above 126, and NaN, something finite above kMost, so
 // that the half is done over with the other form.
 // One pair of exponentials in kFmaExp takes this way in bf16 calls, whose exponential units (16 a
-// clock) are as busy as the products: 2048 tokens at 14336 575 us without, 542 with every 5th pair,
-// 541 to 567 with every 4th to 16th, 604 with every 2nd.
+// clock) are as busy as the products: 2048 tokens at 14336 took 575 us without, 542 with every 5th
+// pair, 541 to 567 with every 4th to 16th, 604 with every 2nd (565 with every 5th now; the error of
+// such calls against 64 bits is 1.68e-3, of which rounding the output alone makes 1.66e-3).
 __device__ __forceinline__ float2 ex2_fma(float2 z) {
     asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(z.x));  // -127, 126
     asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(z.y));
@@ -407,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // One copy of the code and one register set: a tile's words are requested when the tile before
         // is decoded, and have until a stage is given back.  The five roles' loops have to fit the
         // instruction cache together: with two sets in turn (this code twice) a seventh of its requests
-        // missed, and 2048 tokens at 14336 took 626 us where they take 575.
+        // missed, and 2048 tokens at 14336 took 626 us instead of 575.
         auto stream = [&](auto x, auto key, auto fetch, auto decode) {
             int id = id_of(key(0));
             fetch(0, id, x);

@@ -427,11 +427,14 @@ int gb_kv_q4_read(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, void*
 /* Attention of q rows [n][Hq][head_dim] (strides in elements, dims contiguous) over the cache, GQA
  * (Hq a multiple of n_kv_heads): row r sees positions 0 .. min(pos, max_kv - 1) of its sequence,
  * max_kv <= 0: the sequence's whole capacity; a row that sees none (position -1) gets zeros.
- * scale: finite.  Positions on a page outside the pool are not seen.  Values past a row's positions may be
- * anything (NaN included), also where other rows of the call see them.  A seen value whose scale
- * is beyond 8188 in magnitude, which no write stores, may count as NaN.  o: contiguous [n][Hq][head_dim] of q's type.  head_dim 64, 128 or 256.
- * Arithmetic: f32 q to about 1e-6 of fp32 (two-term f16 products, fp32 sums); f16 / bf16 q: V and
- * the probabilities rounded to f16, fp32 sums.  work: gb_kv_q4_attend_workspace_bytes() of device
+ * scale: finite.  Positions on a page outside the pool are not seen.  Values past a row's positions
+ * may be anything (NaN included), also where other rows of the call see them.  A seen value whose scale
+ * is beyond 8188 in magnitude, which no write stores, may count as NaN.
+ * o: contiguous [n][Hq][head_dim] of q's type.  head_dim 64, 128 or 256.
+ * Arithmetic: fp32 sums.  f32 q to about 1e-6 of fp32 (operands in two f16 terms).  f16 q: V rounded
+ * to f16, K exact, the probabilities in two f16 terms (error 2.6e-4 of the output, where rounding it
+ * to f16 makes 2.1e-4).  bf16 q: V, the probabilities and, in chunks, K rounded to f16 (1.7e-3, what
+ * rounding to bf16 makes).  work: gb_kv_q4_attend_workspace_bytes() of device
  * memory (256-byte aligned), its first GB_KV_Q4_WORK_ZEROED bytes zeroed before the first use (every
  * call leaves them zero); calls that can overlap, replays of captured graphs among them, need one
  * each, and memory that a graph has captured has to outlive it. */
@@ -445,7 +448,7 @@ int gb_kv_q4_attend(const gb_kv_q4* cache, const gb_kv_rows* rows, int type, con
  * *step_pos + 1, .. of sequence `slot`, step_pos a device int64 that a captured graph reads anew at
  * each replay, and n_rows consecutive rows.  Arithmetic: chunks that the tensor cores' tiles take
  * (head_dim 64 or 128) round q, K and V to f16 and keep the probabilities in two f16 terms, fp32
- * sums; other calls are as above.  work as for gb_kv_q4_attend. */
+ * sums (error 3.3e-4); other calls are as above.  work as for gb_kv_q4_attend. */
 int gb_kv_q4_attend_prefill(const gb_kv_q4* cache, int64_t n_rows, const int64_t* step_pos,
                             int64_t slot, const float* q, int64_t q_row_stride,
                             int64_t q_head_stride, int64_t Hq, int64_t max_kv, float scale, float* o,
